@@ -28,6 +28,7 @@ CFLAGS = [
     "-fvisibility=hidden",
     "-Wall",
     "-Wno-unused-function",
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",  # scalar FP32 forms only (the host pass ignores it)
     "-munsafe-fp-atomics",  # hardware global_atomic_add_f32 (no CAS loop)
     f"-I{INCLUDE}",         # common.h includes the C-ABI header: definitions are checked against it
 ]
