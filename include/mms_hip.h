@@ -465,6 +465,46 @@ int mms_adamw_dev_multi(int nseg, float* const* p, const float* const* g, float*
                         const int64_t* n, const float* const* sumsq, const float* max_norm, const float* const* hyper,
                         void* stream);
 
+/* ---- Muon's update of weight matrices (an optimizer beside AdamW; torch.optim.Muon's arithmetic): the momentum, its
+ * orthogonalisation by Newton-Schulz products, the weights.  n matrices or stacks of batch[i] matrices of rows[i] x
+ * cols[i] in one call (host tables of device pointers, leading dimensions ld* and distances bs* of a stack's matrices
+ * in elements; last dimension contiguous); p / g / out are fp32 (bf16 = 0) or all bf16 (bf16 = 1), m fp32
+ * [batch, rows, cols] contiguous.  Empty matrices are skipped.
+ *   X = G / max(|G|_F, eps), then `steps` times X <- a X + (b A + c A A) X, A = X X^T, on the side with fewer rows.
+ * The iterates' entries and those of A and b A + c A A must stay below 63 in magnitude (a, b, c = 3.4445, -4.7750,
+ * 2.0315 keep them below 8).  A matrix of zeros gives zeros; one with a NaN or infinity gives NaN.
+ * prec 0: products of split fp16 (fp32's accuracy), 1: fp16 products where a matrix is large (bf16's accuracy).
+ * ws: mms_muon_workspace's bytes (HOST function), 256-byte aligned, used by this call alone while it runs. */
+int mms_muon_workspace(int n, const int64_t* batch, const int64_t* rows, const int64_t* cols, int prec,
+                       int64_t* bytes);
+int mms_newton_schulz(int n, const int64_t* batch, const int64_t* rows, const int64_t* cols, const void* const* g,
+                      const int64_t* ldg, const int64_t* bsg, void* const* out, const int64_t* ldo, const int64_t* bso,
+                      int bf16, int prec, int steps, float a, float b, float c, double eps, void* ws, int64_t ws_bytes,
+                      void* stream);
+/*   m <- m + (1 - momentum)(g' - m), u = g' + momentum (m - g') (nesterov) or m, p <- decay p + neg_lr scale[i] X(u)
+ * with g' = g min(1, max_norm / (sqrt(*sumsq) + 1e-6)) (sumsq NULL: g), decay and neg_lr read from device hyper[2] if
+ * it is given (graph replays).  Same in every other respect. */
+int mms_muon_step(int n, const int64_t* batch, const int64_t* rows, const int64_t* cols, void* const* p,
+                  const int64_t* ldp, const int64_t* bsp, const void* const* g, const int64_t* ldg, const int64_t* bsg,
+                  float* const* m, const float* scale, int bf16, int prec, int steps, float a, float b, float c,
+                  double eps, double momentum, int nesterov, const float* sumsq, float max_norm, const float* hyper,
+                  float decay, float neg_lr, void* ws, int64_t ws_bytes, void* stream);
+
+/* ---- learned row tables (a learned table of an index beside the hash grid's of a position: per-view or per-token
+ * codes).  out[i, :] = scale table[ids[i], :], ids [n] int32 or int64 (ids64) ids_stride elements apart, table [rows,
+ * ldt], out [n, ldo]; dtype of table, out and gradients: 0 fp32, 1 bf16, 2 fp16.  An index outside the table gives a row
+ * of zeros. */
+int mms_embedding_fwd(const void* ids, int ids64, int64_t ids_stride, int64_t n, const void* table, int64_t ldt,
+                      int64_t rows, int dim, int dtype, float scale, void* out, int64_t ldo, void* stream);
+/* dtable[v, :] = scale sum over ids[i] = v of dout[i, :] for every row v (accumulate: +=, rows that do not occur stay as
+ * they are); positions whose index is padding_idx or outside the table add nothing, whatever dout holds there.  Sums in
+ * fp32 in an order fixed by ids alone: the same bits on each call.  ws: mms_embedding_bwd_workspace's bytes (HOST
+ * function), 256-byte aligned, used by this call alone while it runs. */
+int mms_embedding_bwd_workspace(int64_t n, int64_t rows, int dim, int dtype, int64_t* bytes);
+int mms_embedding_bwd(const void* ids, int ids64, int64_t ids_stride, int64_t n, const void* dout, int64_t ldd,
+                      int64_t rows, int dim, int dtype, float scale, int64_t padding_idx, void* dtable, int64_t ldg,
+                      int accumulate, void* ws, int64_t ws_bytes, void* stream);
+
 /* ---- GPU-resident uniform pixel sampler (UniformPixelSampler.sample, cameras/pixel_samplers.py:71-89, over the
  * frames CacheDataloader caches, data/dataloaders.py:107-167): n draws of (frame, x, y) from Philox4x32-10
  * (key seed, counter *counter + i, stream_id; *counter += n on the device afterwards, so graph replays advance it).

@@ -218,3 +218,274 @@ def gemm_tn_wide16(items, target_blocks: Optional[int] = None):
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+# ----------------------------------------------------------------------------------------------
+# Muon: orthogonalised updates of weight matrices
+# ----------------------------------------------------------------------------------------------
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # torch.optim.Muon's quintic
+_MATRIX_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+class _on_device:
+    """The device of ``t`` as the current one (a no-op if it is already): streams and launches go to it."""
+
+    def __init__(self, t: torch.Tensor):
+        self.guard = None if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _matrices(t: torch.Tensor, what: str, copy: bool):
+    """(tensor, batch, rows, cols, leading dimension, distance of a stack's matrices) of [..., rows, cols]; a layout
+    that the kernels do not read in place is copied if ``copy``, else refused."""
+    if t.dim() < 2:
+        raise ValueError(f"{what} must have at least two dimensions, got shape {tuple(t.shape)}")
+    rows, cols = t.shape[-2:]
+
+    def in_place(x):
+        return x.numel() == 0 or ((cols == 1 or x.stride(-1) == 1) and (rows == 1 or x.stride(-2) >= cols))
+    if not in_place(t):
+        if not copy:
+            raise ValueError(f"{what}: rows must be contiguous and not overlap, got strides {t.stride()}")
+        t = t.contiguous()
+    if t.dim() > 3:
+        t = t.reshape(-1, rows, cols) if copy else t.view(-1, rows, cols)
+    ld = cols if rows == 1 else t.stride(-2)
+    batch = t.shape[0] if t.dim() == 3 else 1
+    bs = 0 if batch <= 1 else t.stride(0)
+    if batch > 1 and t.numel() and bs < (rows - 1) * ld + cols:
+        if not copy:
+            raise ValueError(f"{what}: stacked matrices must not overlap, got strides {t.stride()}")
+        t = t.contiguous()
+        ld, bs = cols, rows * cols
+    return t, batch, rows, cols, ld, bs
+
+
+class _MatrixTable:
+    """Host tables of several matrices for mms_newton_schulz / mms_muon_step."""
+
+    def __init__(self, mats):
+        n = self.n = len(mats)
+        I64, VP = ctypes.c_int64 * n, ctypes.c_void_p * n
+        self.keep = [m[0] for m in mats]
+        self.batch, self.rows, self.cols = (I64(*[m[i] for m in mats]) for i in (1, 2, 3))
+        self.ptr = VP(*[m[0].data_ptr() for m in mats])
+        self.ld, self.bs = I64(*[m[4] for m in mats]), I64(*[m[5] for m in mats])
+
+
+def _muon_workspace(tab: _MatrixTable, prec: int, device) -> torch.Tensor:
+    need = ctypes.c_int64(0)
+    _lib.call("mms_muon_workspace", tab.n, tab.batch, tab.rows, tab.cols, int(prec), ctypes.addressof(need))
+    return torch.empty(max(1, need.value), dtype=torch.uint8, device=device)
+
+
+def _check_matrices(ts, what: str):
+    _check_dev(*ts)
+    for t in ts:
+        if t.dtype not in _MATRIX_DTYPES:
+            raise TypeError(f"{what} must be float32 or bfloat16, got {t.dtype}")
+        if t.device != ts[0].device:
+            raise ValueError(f"{what} must be on one device, got {ts[0].device} and {t.device}")
+
+
+def _prec_of(dtype, prec: Optional[int]) -> int:
+    return (0 if dtype == torch.float32 else 1) if prec is None else int(prec)
+
+
+def newton_schulz(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7, prec: Optional[int] = None):
+    """The nearest semi-orthogonal matrix, approximately, of each matrix by Newton-Schulz products:
+    X = G / max(|G|_F, eps), then ``steps`` times X <- a X + (b A + c A A) X with A = X X^T (X^T X for tall G) -- the
+    iteration of torch.optim.Muon.
+
+    ``mats``: a tensor [..., rows, cols] (a stack of matrices) or a list of such; float32 or bfloat16; returns the
+    same structure, contiguous.  ``prec``: 0 fp32's accuracy (float32's default), 1 bfloat16's (its default).  A zero
+    matrix gives zeros, one with NaN or infinities NaN.  All matrices share the same few launches."""
+    if isinstance(mats, torch.Tensor):
+        return newton_schulz([mats], steps, coefficients, eps, prec)[0]
+    mats = list(mats)
+    _check_matrices(mats, "newton_schulz: matrices")
+    a, b, c = (float(x) for x in coefficients)
+    outs = [torch.empty(m.shape, dtype=m.dtype, device=m.device) for m in mats]
+    for dtype, bf16 in _MATRIX_DTYPES.items():
+        pick = [i for i, m in enumerate(mats) if m.dtype == dtype]
+        if not pick:
+            continue
+        p = _prec_of(dtype, prec)
+        with _on_device(mats[0]):
+            g = _MatrixTable([_matrices(mats[i], "newton_schulz: matrix", True) for i in pick])
+            o = _MatrixTable([_matrices(outs[i], "newton_schulz: result", False) for i in pick])
+            ws = _muon_workspace(g, p, mats[0].device)
+            _lib.call("mms_newton_schulz", g.n, g.batch, g.rows, g.cols, g.ptr, g.ld, g.bs, o.ptr, o.ld, o.bs, bf16, p,
+                      int(steps), a, b, c, float(eps), ws.data_ptr(), ws.numel(), _stream())
+    return outs
+
+
+def muon_scale(rows: int, cols: int, adjust: Optional[str] = None) -> float:
+    """The learning rate's factor for a rows x cols matrix (torch.optim.Muon's adjust_lr_fn)."""
+    if adjust in (None, "original"):
+        return max(1.0, rows / max(1, cols)) ** 0.5
+    if adjust == "match_rms_adamw":
+        return 0.2 * max(rows, cols) ** 0.5
+    raise ValueError(f"adjust must be 'original' or 'match_rms_adamw', got {adjust!r}")
+
+
+def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nesterov: bool = True,
+              weight_decay: float = 0.1, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7,
+              adjust: Optional[str] = None, prec: Optional[int] = None, sumsq: Optional[torch.Tensor] = None,
+              max_norm: float = 0.0, hyper: Optional[torch.Tensor] = None) -> None:
+    """One Muon step of weight matrices, in place:
+    m <- m + (1 - momentum)(g - m), u = g + momentum (m - g) (``nesterov``) or m,
+    p <- (1 - lr weight_decay) p - lr scale newton_schulz(u), scale = ``muon_scale(rows, cols, adjust)``.
+
+    ``params`` / ``grads``: lists of [..., rows, cols] tensors of one type each, float32 or bfloat16; ``momenta``:
+    float32, contiguous, zeros before the first step.  ``sumsq`` (device, one float) with ``max_norm``: the gradients
+    are clipped by min(1, max_norm / (sqrt(sumsq) + 1e-6)).  ``hyper`` (device): [1 - lr weight_decay, -lr] read by the
+    kernels in place of the arguments (graph replays)."""
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    if not len(params) == len(grads) == len(momenta):
+        raise ValueError(f"muon_step: {len(params)} weights, {len(grads)} gradients, {len(momenta)} momenta")
+    if not params:
+        return
+    _check_matrices(params, "muon_step: weights")
+    _check_dev(*grads, *momenta, sumsq, hyper)
+    for p, g, m in zip(params, grads, momenta):
+        if g.shape != p.shape or m.shape != p.shape:
+            raise ValueError(f"muon_step: weights {tuple(p.shape)}, gradient {tuple(g.shape)}, momentum "
+                             f"{tuple(m.shape)} must have one shape")
+        if g.dtype != p.dtype or m.dtype != torch.float32 or not m.is_contiguous():
+            raise ValueError("muon_step: gradients have their weights' type, momenta are contiguous float32")
+        if g.device != p.device or m.device != p.device:
+            raise ValueError("muon_step: weights, gradients and momenta must be on one device")
+    for what, ts in (("weights", params), ("momenta", momenta)):
+        if len({t.data_ptr() for t in ts if t.numel()}) < sum(1 for t in ts if t.numel()):
+            raise ValueError(f"muon_step: the same {what} twice")
+    for t, k in ((sumsq, 1), (hyper, 2)):
+        if t is not None and (t.dtype != torch.float32 or t.numel() < k or not t.is_contiguous()
+                              or t.device != params[0].device):
+            raise ValueError("muon_step: sumsq and hyper are contiguous float32 on the weights' device")
+    a, b, c = (float(x) for x in coefficients)
+    for dtype, bf16 in _MATRIX_DTYPES.items():
+        pick = [i for i, p in enumerate(params) if p.dtype == dtype]
+        if not pick:
+            continue
+        pr = _prec_of(dtype, prec)
+        with torch.no_grad(), _on_device(params[0]):
+            w = _MatrixTable([_matrices(params[i].detach(), "muon_step: weights", False) for i in pick])
+            g = _MatrixTable([_matrices(grads[i].detach(), "muon_step: gradient", True) for i in pick])
+            m = (ctypes.c_void_p * w.n)(*[momenta[i].data_ptr() for i in pick])
+            scale = (ctypes.c_float * w.n)(*[muon_scale(w.rows[k], w.cols[k], adjust) for k in range(w.n)])
+            ws = _muon_workspace(w, pr, params[0].device)
+            _lib.call("mms_muon_step", w.n, w.batch, w.rows, w.cols, w.ptr, w.ld, w.bs, g.ptr, g.ld, g.bs, m, scale,
+                      bf16, pr, int(steps), a, b, c, float(eps), float(momentum), int(bool(nesterov)), _ptr(sumsq),
+                      float(max_norm), _ptr(hyper), 1.0 - float(lr) * float(weight_decay), -float(lr), ws.data_ptr(),
+                      ws.numel(), _stream())
+
+
+# ----------------------------------------------------------------------------------------------
+# learned row tables
+# ----------------------------------------------------------------------------------------------
+_TABLE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _check_table(ids: torch.Tensor, rows: torch.Tensor, what: str):
+    _check_dev(ids, rows)
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"embedding: indices must be int32 or int64, got {ids.dtype}")
+    if rows.dtype not in _TABLE_DTYPES:
+        raise TypeError(f"embedding: {what} must be float32, bfloat16 or float16, got {rows.dtype}")
+    if ids.device != rows.device:
+        raise ValueError(f"embedding: indices on {ids.device}, {what} on {rows.device}")
+
+
+def _flat_ids(ids: torch.Tensor):
+    """(tensor, elements between two indices): a column of a coordinate tensor is read where it lies."""
+    n = ids.numel()
+    if ids.is_contiguous():
+        return ids, 1
+    lead = [(s, st) for s, st in zip(ids.shape, ids.stride()) if s != 1]
+    if n and len(lead) == 1 and lead[0][1] > 0:
+        return ids, lead[0][1]
+    return ids.contiguous(), 1
+
+
+def _rows2d(t: torch.Tensor, dim: int) -> torch.Tensor:
+    t = t.reshape(-1, dim)
+    return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= dim) else t.contiguous()
+
+
+def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """out[..., :] = scale * table[ids[...], :]; ids int32 / int64 of any shape, table [rows, dim] float32, bfloat16 or
+    float16.  An index outside the table gives a row of zeros."""
+    _check_table(ids, table, "the table")
+    if table.dim() != 2 or table.shape[0] == 0 or table.shape[1] == 0:
+        raise ValueError(f"embedding: the table must be [rows, dim], got {tuple(table.shape)}")
+    t = table if table.stride(1) == 1 and table.stride(0) >= table.shape[1] else table.contiguous()
+    out = torch.empty(*ids.shape, table.shape[1], dtype=table.dtype, device=table.device)
+    flat, stride = _flat_ids(ids)
+    with _on_device(t):
+        _lib.call("mms_embedding_fwd", flat.data_ptr(), int(ids.dtype == torch.int64), stride, ids.numel(),
+                  t.data_ptr(), t.stride(0), t.shape[0], t.shape[1], _TABLE_DTYPES[t.dtype], float(scale),
+                  out.data_ptr(), t.shape[1], _stream())
+    return out
+
+
+def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: float = 1.0,
+                       padding_idx: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                       accumulate: bool = False) -> torch.Tensor:
+    """The table's gradient [rows, dim] in ``dout``'s type: scale * the sum of dout over the positions of each row, in
+    fp32 and in an order that ``ids`` alone fixes (the same bits on each call).  Positions whose index is
+    ``padding_idx`` or outside the table add nothing, whatever ``dout`` holds there.  ``out``: written in place, or
+    added into with ``accumulate``."""
+    _check_table(ids, dout, "the gradient")
+    dim = dout.shape[-1] if dout.dim() else 0
+    if dim == 0 or tuple(dout.shape[:-1]) != tuple(ids.shape) or rows < 1:
+        raise ValueError(f"embedding_backward: indices {tuple(ids.shape)} need a gradient [..., dim], got "
+                         f"{tuple(dout.shape)} for {rows} rows")
+    if out is None:
+        if accumulate:
+            raise ValueError("embedding_backward: accumulate needs out")
+        out = torch.empty(rows, dim, dtype=dout.dtype, device=dout.device)
+    elif tuple(out.shape) != (rows, dim) or out.dtype != dout.dtype or out.device != dout.device or \
+            (dim > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < dim):
+        raise ValueError(f"embedding_backward: out must be [{rows}, {dim}] {dout.dtype} with contiguous rows on "
+                         f"{dout.device}")
+    if padding_idx is not None:
+        if not -rows <= padding_idx < rows:
+            raise ValueError(f"embedding_backward: padding_idx {padding_idx} is outside the table's {rows} rows")
+        padding_idx = padding_idx % rows
+    d = _rows2d(dout, dim)
+    flat, stride = _flat_ids(ids)
+    dt = _TABLE_DTYPES[dout.dtype]
+    need = ctypes.c_int64(0)
+    _lib.call("mms_embedding_bwd_workspace", ids.numel(), int(rows), dim, dt, ctypes.addressof(need))
+    with _on_device(dout):
+        ws = torch.empty(max(1, need.value), dtype=torch.uint8, device=dout.device)
+        _lib.call("mms_embedding_bwd", flat.data_ptr(), int(ids.dtype == torch.int64), stride, ids.numel(),
+                  d.data_ptr(), dim if d.shape[0] <= 1 else d.stride(0), int(rows), dim, dt, float(scale),
+                  -1 if padding_idx is None else int(padding_idx), out.data_ptr(), dim if rows == 1 else out.stride(0),
+                  int(bool(accumulate)), ws.data_ptr(), ws.numel(), _stream())
+    return out
+
+
+class EmbeddingFunction(torch.autograd.Function):
+    """Learned row table forward / backward on the HIP kernels: apply(ids, table, scale=1.0, padding_idx=None)."""
+
+    @staticmethod
+    def forward(ctx, ids, table, scale: float = 1.0, padding_idx: Optional[int] = None):
+        ctx.save_for_backward(ids)
+        ctx.cfg = (table.shape[0], float(scale), padding_idx)
+        return embedding(ids, table, scale)
+
+    @staticmethod
+    def backward(ctx, dout):
+        (ids,) = ctx.saved_tensors
+        rows, scale, padding_idx = ctx.cfg
+        dtable = embedding_backward(ids, dout, rows, scale, padding_idx) if ctx.needs_input_grad[1] else None
+        return None, dtable, None, None

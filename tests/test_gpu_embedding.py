@@ -1,0 +1,192 @@
+"""Learned row tables (hip_ops.embedding, embedding_backward, EmbeddingFunction) against plain sums in 64 bits.
+
+Tolerances.  The lookup is one float32 product rounded once: the same bits as torch's.  A gradient is a float32 sum of
+k values: off by at most k half steps (2^-24 each, one more for the scale) of the sum of the values' magnitudes, and by
+a half step of the result's type."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}
+DTYPES = list(HALF)
+
+
+@pytest.fixture()
+def gen(dev):
+    return torch.Generator(device="cuda").manual_seed(23)
+
+
+def plain_sums(ids, dout, rows, scale, pad=None):
+    """(gradient, bound on |error|) in 64 bits."""
+    ids, d = ids.reshape(-1).long(), dout.reshape(-1, dout.shape[-1]).double()
+    live = (ids >= 0) & (ids < rows)
+    if pad is not None:
+        live &= ids != pad
+    ids, d = ids[live], d[live]
+    want = torch.zeros(rows, d.shape[1], dtype=torch.float64, device=d.device).index_add_(0, ids, d) * scale
+    mag = torch.zeros_like(want).index_add_(0, ids, d.abs()) * abs(scale)
+    count = torch.bincount(ids, minlength=rows)[:, None]
+    return want, (count + 1) * 2.0 ** -24 * mag + HALF[dout.dtype] * want.abs() + TINY[dout.dtype]
+
+
+def check(got, ids, dout, rows, scale=1.0, pad=None, base=None):
+    want, tol = plain_sums(ids, dout, rows, scale, pad)
+    if base is not None:
+        want = want + base.double()
+        tol = tol + (2.0 ** -24 + HALF[dout.dtype]) * want.abs()
+    assert got.shape == want.shape and got.dtype == dout.dtype
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist())
+
+
+def draw_ids(kind, n, rows, gen):
+    if kind == "same":
+        return torch.full((n,), rows // 2, device="cuda")
+    if kind == "sorted":
+        return torch.arange(n, device="cuda") * rows // max(n, 1)
+    if kind == "reversed":
+        return rows - 1 - torch.arange(n, device="cuda") % rows
+    if kind == "skewed":
+        return (torch.rand(n, device="cuda", generator=gen) ** 8 * rows).long()
+    if kind == "outside":
+        return torch.randint(-3, rows + 3, (n,), device="cuda", generator=gen)
+    return torch.randint(0, rows, (n,), device="cuda", generator=gen)
+
+
+# n: none, around a run's length, a one-block sort's end (12288), several blocks, more than 64 of them; rows: one and
+# two sort digits and their borders, three digits; dim: one value, below / over 16 bytes, one and more column segments
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n,rows,dim,kind", [
+    (0, 7, 8, "uniform"), (1, 1, 1, "same"), (1, 5, 4100, "uniform"), (2, 2, 3, "reversed"), (63, 9, 16, "uniform"),
+    (64, 1, 8, "same"), (65, 130, 64, "sorted"), (1000, 45, 32, "uniform"), (1000, 3, 2050, "skewed"),
+    (4096, 1023, 24, "uniform"), (5000, 1024, 40, "outside"), (12288, 45, 32, "skewed"), (12289, 45, 32, "skewed"),
+    (9001, 50257, 77, "skewed"), (20000, 2000, 771, "uniform"), (40000, 5, 64, "same"), (40000, 300, 96, "reversed"),
+    (30000, 131072, 256, "skewed"), (300000, 1000, 8, "skewed"), (270000, 2097153, 2, "outside"),
+])
+def test_lookup_and_gradient(dev, gen, n, rows, dim, kind, dtype):
+    from multimodalstudio_amd import hip_ops
+    ids = draw_ids(kind, n, rows, gen)
+    table = torch.randn(rows, dim, device="cuda", generator=gen).to(dtype)
+    out = hip_ops.embedding(ids, table, 1.7)
+    live = ((ids >= 0) & (ids < rows))[:, None]
+    want = torch.where(live, (table[ids.clamp(0, rows - 1)].float() * 1.7).to(dtype), torch.zeros((), dtype=dtype, device="cuda"))
+    assert torch.equal(out, want)
+    dout = torch.randn(n, dim, device="cuda", generator=gen).to(dtype)
+    got = hip_ops.embedding_backward(ids, dout, rows, 0.6)
+    check(got, ids, dout, rows, 0.6)
+    assert torch.equal(got, hip_ops.embedding_backward(ids.int(), dout, rows, 0.6))
+
+
+@pytest.mark.parametrize("n", [1000, 20000])
+def test_padding_hides_what_its_positions_hold(dev, gen, n):
+    """NaN and infinities in the gradient of padded and outside positions reach nothing; all padding gives zeros."""
+    from multimodalstudio_amd import hip_ops
+    ids = torch.randint(0, 50, (n,), device="cuda", generator=gen)
+    ids[::7] = 12
+    ids[3::11] = 50
+    dout = torch.randn(n, 33, device="cuda", generator=gen)
+    clean = dout.clone()
+    dout[(ids == 12) | (ids == 50)] = float("nan")
+    clean[(ids == 12) | (ids == 50)] = 0.0
+    got = hip_ops.embedding_backward(ids, dout, 50, padding_idx=12)
+    check(got, ids, clean, 50, 1.0, 12)
+    assert (got[12] == 0).all() and torch.equal(got, hip_ops.embedding_backward(ids, dout, 50, padding_idx=12 - 50))
+    ids.fill_(12)
+    assert (hip_ops.embedding_backward(ids, dout, 50, padding_idx=12) == 0).all()
+    with pytest.raises(ValueError):
+        hip_ops.embedding_backward(ids, dout, 50, padding_idx=50)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("n,rows,dim", [(500, 40, 32), (30000, 300, 5), (20000, 9, 64)])
+def test_accumulate_and_layouts(dev, gen, dtype, n, rows, dim):
+    """Added into rows of a wider, misaligned buffer; a gradient that is a slice of a wider one; indices that are a
+    column of coordinates, in more dimensions than one.  What lies beside the rows stays."""
+    from multimodalstudio_amd import hip_ops
+    coords = torch.randint(0, rows, (n, 3), device="cuda", generator=gen, dtype=torch.int32)
+    coords[:, 0] = coords[:, 0] // 2 * 2       # odd rows do not occur
+    buf = torch.randn(rows, dim + 9, device="cuda", generator=gen).to(dtype)
+    keep = buf.clone()
+    out = buf[:, 1:1 + dim]
+    dout = torch.randn(n, dim + 3, device="cuda", generator=gen).to(dtype)[:, 2:2 + dim]
+    r = hip_ops.embedding_backward(coords[:, 0], dout, rows, 0.5, out=out, accumulate=True)
+    assert r is out
+    check(out, coords[:, 0], dout, rows, 0.5, None, keep[:, 1:1 + dim])
+    assert torch.equal(buf[1::2], keep[1::2]) and torch.equal(buf[:, :1], keep[:, :1])
+    assert torch.equal(buf[:, 1 + dim:], keep[:, 1 + dim:])
+    hip_ops.embedding_backward(coords[:, :1], dout[:, None], rows, 0.5, out=out)
+    check(out, coords[:, 0], dout, rows, 0.5)
+    assert (out[1::2] == 0).all() and torch.equal(buf[:, 1 + dim:], keep[:, 1 + dim:])
+    table = buf[:, 3:3 + dim]
+    got = hip_ops.embedding(coords[:, :2], table)
+    assert got.shape == (n, 2, dim) and torch.equal(got, table[coords[:, :2].long()])
+    got = hip_ops.embedding(coords[:, 1:2], table)
+    assert torch.equal(got, table[coords[:, 1:2].long()])
+
+
+def test_refusals(dev):
+    from multimodalstudio_amd import hip_ops
+    ids, t = torch.zeros(4, dtype=torch.int64, device="cuda"), torch.zeros(5, 8, device="cuda")
+    d = torch.zeros(4, 8, device="cuda")
+    for bad in (lambda: hip_ops.embedding(ids.float(), t), lambda: hip_ops.embedding(ids, t.double()),
+                lambda: hip_ops.embedding_backward(ids, d.double(), 5)):
+        with pytest.raises(TypeError):
+            bad()
+    for bad in (lambda: hip_ops.embedding(ids, t[0]), lambda: hip_ops.embedding(ids, t[:0]),
+                lambda: hip_ops.embedding_backward(ids[:3], d, 5), lambda: hip_ops.embedding_backward(ids, d, 0),
+                lambda: hip_ops.embedding_backward(ids, d, 5, accumulate=True),
+                lambda: hip_ops.embedding_backward(ids, d, 5, out=t[:4]),
+                lambda: hip_ops.embedding_backward(ids, d, 5, out=t.bfloat16()),
+                lambda: hip_ops.embedding_backward(ids, d, 5, out=torch.zeros(8, 5, device="cuda").mT)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError, match="device"):
+        hip_ops.embedding(ids.cpu(), t)
+
+
+def test_function_gradient(dev, gen):
+    """Autograd's gradient of a loss over looked-up rows: the formula's, and differences of the loss (a quadratic, so
+    central differences are exact up to rounding: float32 losses near 1 are off by 2^-23, over a step of 2 * 0.25)."""
+    from multimodalstudio_amd.hip_ops import EmbeddingFunction
+    ids = torch.randint(0, 6, (4, 10), device="cuda", generator=gen)
+    table = (0.1 * torch.randn(6, 5, device="cuda", generator=gen)).requires_grad_()
+    w = 0.1 * torch.randn(4, 10, 5, device="cuda", generator=gen)
+
+    def loss(t):
+        y = EmbeddingFunction.apply(ids, t, 2.0, 3)
+        return (w * y + 0.05 * y * y).double().sum()
+    loss(table).backward()
+    y = 2.0 * table.detach()[ids].double()
+    check(table.grad, ids, (w.double() + 0.1 * y).float(), 6, 2.0, 3)
+    with torch.no_grad():
+        for v, c in ((0, 0), (2, 4), (5, 1)):
+            up, down = table.detach().clone(), table.detach().clone()
+            up[v, c] += 0.25
+            down[v, c] -= 0.25
+            diff = float(loss(up) - loss(down)) / 0.5
+            assert abs(diff - float(table.grad[v, c])) <= 1e-4
+    assert (table.grad[3] == 0).all()
+
+
+@pytest.mark.parametrize("n", [3000, 30000])
+def test_in_a_graph(dev, gen, n):
+    """Lookup and gradient captured once, replayed on new indices between eager calls: the eager results' bits."""
+    from multimodalstudio_amd import hip_ops
+    table = torch.randn(900, 64, device="cuda", generator=gen)
+    ids = torch.zeros(n, dtype=torch.int64, device="cuda")
+    dout = torch.zeros(n, 64, device="cuda")
+    hip_ops.embedding_backward(ids, dout, 900)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = hip_ops.embedding(ids, table, 0.5)
+        grad = hip_ops.embedding_backward(ids, dout, 900, 0.5)
+    for k in range(4):
+        ids.copy_(draw_ids(["uniform", "skewed", "same", "outside"][k], n, 900, gen))
+        dout.normal_(generator=gen)
+        graph.replay()
+        a, b = hip_ops.embedding(ids, table, 0.5), hip_ops.embedding_backward(ids, dout, 900, 0.5)
+        torch.cuda.synchronize()
+        assert torch.equal(out, a) and torch.equal(grad, b)
