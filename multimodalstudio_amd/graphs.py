@@ -197,9 +197,8 @@ class GraphTrainer:
             t.optim.zero_grads(extra)
             fx.zero_arena_begin(t.device, zeroed=arena)
         else:
-            t.fields.zero_grad()
-            if t.poses is not None:
-                t.poses.zero_grad()
+            for g in t.groups:
+                g.zero_grad()
             fx.zero_arena_begin(t.device)
         try:
             return self._forward_backward_body(t, targets, cap, between, mid)
@@ -284,9 +283,8 @@ class GraphTrainer:
         if BANKED_OPTIM:
             t.optim.step_captured()
             return
-        t.fields.step_captured()
-        if t.poses is not None:
-            t.poses.step_captured()
+        for g in t.groups:
+            g.step_captured()
 
     def capture(self, key: tuple) -> None:
         cap = key[0]
@@ -324,17 +322,15 @@ class GraphTrainer:
         if BANKED_OPTIM:
             t.optim.load_hyper(f)
         else:
-            t.fields.load_hyper(f)
-            if t.poses is not None:
-                t.poses.load_hyper(f)
+            for g in t.groups:
+                g.load_hyper(f)
         self.hyper_step = t.step
 
     def _drop_queued_hyper(self):
         """An eager step follows a queued scalar upload: undo its step-count advance (the eager optimizer advances)."""
         if self.hyper_step is not None:
-            self.t.fields.step_count -= 1
-            if self.t.poses is not None:
-                self.t.poses.step_count -= 1
+            for g in self.t.groups:
+                g.step_count -= 1
             self.hyper_step = None
 
     def eager_step(self, coords):
@@ -399,7 +395,7 @@ class GraphTrainer:
             # the rest follows, then the optimizer graph
             g1[0].replay()
             self.ddp.overlap_exchange([(self.table_grads(1), g1[1].replay), (self.table_grads(2), g1[2].replay)],
-                                      [t.fields] + ([t.poses] if t.poses is not None else []))
+                                      t.groups)
             g2.replay()
         if self.tail:
             self.count_event.record()

@@ -20,6 +20,7 @@ from torch import nn
 
 from . import _lib
 from . import functions as fx
+from . import hip_ops
 from . import scene as mscene
 from .model import RNG, BaseModel, ModelSpec
 
@@ -181,12 +182,16 @@ class FlatGroup:
 
     def load_hyper(self, lr_factor: float):
         """Graph mode, before a replay: advance the step and upload its scalars (read by the captured launch)."""
-        lr = self._advance(lr_factor)
         host = self._hyper_host[self._hyper_slot]
         self._hyper_slot ^= 1
+        self.write_hyper(lr_factor, host)
+        self.hyper.copy_(host, non_blocking=True)
+
+    def write_hyper(self, lr_factor: float, host: torch.Tensor):
+        """Advance the step and write its scalars to 8 host floats (the layout the captured launch reads)."""
+        lr = self._advance(lr_factor)
         _lib.call("mms_adamw_scalars", float(lr), float(self.wd), float(self.betas[0]), float(self.betas[1]),
                   float(self.eps), int(self.step_count), host.data_ptr())
-        self.hyper.copy_(host, non_blocking=True)
 
     def step_captured(self, max_norm: float = 2.0):
         """The clip + AdamW launches with device-resident scalars (captured into the step graph)."""
@@ -195,6 +200,56 @@ class FlatGroup:
         _lib.call("mms_sumsq", self.grad.data_ptr(), self.n, self.sumsq.data_ptr(), _s())
         _lib.call("mms_adamw_dev", self.flat.data_ptr(), self.grad.data_ptr(), self.m.data_ptr(), self.v.data_ptr(),
                   self.n, self.sumsq.data_ptr(), float(max_norm), self.hyper.data_ptr(), _s())
+
+
+class MuonGroup(FlatGroup):
+    """Weight matrices stepped by Muon (hip_ops.muon_step) in place of AdamW: the same flat buffers, clip and schedule;
+    ``m`` is the momentum and there is no second moment.  The learning rate's factor per matrix is
+    ``hip_ops.muon_scale``: with "match_rms_adamw" an AdamW group's lr and weight_decay carry over."""
+
+    def __init__(self, params: List[nn.Parameter], lr: float, weight_decay: float, momentum: float = 0.95,
+                 nesterov: bool = True, steps: int = 5, coefficients=hip_ops.NS_COEFFICIENTS, eps: float = 1e-7,
+                 adjust: Optional[str] = "match_rms_adamw"):
+        params = list(params)
+        for p in params:
+            if p.dim() != 2 or p.dtype != torch.float32:
+                raise ValueError(f"MuonGroup holds float32 matrices, got {p.dtype} {tuple(p.shape)}")
+        super().__init__(params, lr, weight_decay, eps)
+        self.v = None
+        self.momentum, self.nesterov, self.steps = float(momentum), bool(nesterov), int(steps)
+        self.coefficients, self.adjust = tuple(float(c) for c in coefficients), adjust
+        off, self.momenta = 0, []
+        for p in self.params:
+            self.momenta.append(self.m[off:off + p.numel()].view_as(p))
+            off += p.numel()
+
+    def _muon(self, max_norm: float, **scalars):
+        self.sumsq_of_grads()
+        self.update(max_norm, **scalars)
+
+    def sumsq_of_grads(self):
+        self.check_grads_attached()
+        self.sumsq.zero_()
+        _lib.call("mms_sumsq", self.grad.data_ptr(), self.n, self.sumsq.data_ptr(), _s())
+
+    def update(self, max_norm: float, **scalars):
+        """The Muon launches on the gradients and their sum of squares."""
+        hip_ops.muon_step([p.data for p in self.params], [p.grad for p in self.params], self.momenta,
+                          momentum=self.momentum, nesterov=self.nesterov, steps=self.steps,
+                          coefficients=self.coefficients, eps=self.eps, adjust=self.adjust, sumsq=self.sumsq,
+                          max_norm=float(max_norm), **scalars)
+
+    def step(self, lr_factor: float, max_norm: float = 2.0):
+        """clip_grad_norm_(max_norm) then the Muon step."""
+        self._muon(max_norm, lr=self._advance(lr_factor), weight_decay=self.wd)
+
+    def write_hyper(self, lr_factor: float, host: torch.Tensor):
+        lr = self._advance(lr_factor)
+        host[0], host[1] = 1.0 - lr * self.wd, -lr
+
+    def step_captured(self, max_norm: float = 2.0):
+        """The clip + Muon launches with device-resident scalars (captured into the step graph)."""
+        self._muon(max_norm, lr=0.0, hyper=self.hyper)
 
 
 ZERO_MULTI_MAX = 8      # buffers per mms_zero_multi launch (kMaxSeg, csrc/loss_optim.hip)
@@ -222,6 +277,10 @@ class OptimBank:
         gs = self.groups
         self._sum = (G, VP(*[g.grad.data_ptr() for g in gs]), I64(*[g.n for g in gs]),
                      VP(*[g.sumsq.data_ptr() for g in gs]))
+        self.muon = [g for g in gs if isinstance(g, MuonGroup)]
+        gs = [g for g in gs if not isinstance(g, MuonGroup)]
+        G = len(gs)
+        I64, VP, F32 = ctypes.c_int64 * G, ctypes.c_void_p * G, ctypes.c_float * G
         self._args = [G, VP(*[g.flat.data_ptr() for g in gs]), VP(*[g.grad.data_ptr() for g in gs]),
                       VP(*[g.m.data_ptr() for g in gs]), VP(*[g.v.data_ptr() for g in gs]), I64(*[g.n for g in gs]),
                       VP(*[g.sumsq.data_ptr() for g in gs]), None, VP(*[g.hyper.data_ptr() for g in gs])]
@@ -246,20 +305,21 @@ class OptimBank:
         host = self._hyper_host[self._hyper_slot]
         self._hyper_slot ^= 1
         for i, g in enumerate(self.groups):
-            lr = g._advance(lr_factor)
-            _lib.call("mms_adamw_scalars", float(lr), float(g.wd), float(g.betas[0]), float(g.betas[1]),
-                      float(g.eps), int(g.step_count), host.data_ptr() + 32 * i)
+            g.write_hyper(lr_factor, host[8 * i:8 * i + 8])
         self.hyper.copy_(host, non_blocking=True)
 
     def step_captured(self, max_norm: float = 2.0):
-        """clip_grad_norm_(max_norm) + AdamW of every group with device-resident scalars (two launches), the
-        accumulators zeroed by zero_grads at the step's start."""
+        """clip_grad_norm_(max_norm) + AdamW of every group with device-resident scalars (two launches; Muon groups by
+        their own), the accumulators zeroed by zero_grads at the step's start."""
         for g in self.groups:
             g.check_grads_attached()
         _lib.call("mms_sumsq_multi", *self._sum, _s())
-        args = list(self._args)
-        args[7] = self._F32(*[float(max_norm)] * len(self.groups))
-        _lib.call("mms_adamw_dev_multi", *args, _s())
+        if self._args[0]:
+            args = list(self._args)
+            args[7] = self._F32(*[float(max_norm)] * args[0])
+            _lib.call("mms_adamw_dev_multi", *args, _s())
+        for g in self.muon:
+            g.update(max_norm, lr=0.0, hyper=g.hyper)
 
 
 def lr_factor(step: int, max_iters: int = 100000, warm_up_ratio=0.1, milestones=(0.5, 0.75, 0.9), gamma=0.4):
@@ -417,6 +477,7 @@ class TrainConfig:
     skip_views: Optional[Dict[str, List[int]]] = None   # skip_image_indices_per_modality (datamanager config)
     data_dir: Optional[str] = None      # an on-disk MMS-DATA scene (data.MMSDataset) instead of the analytic one
     gpu_sampler: bool = False           # draw pixels on the device (data.GPUPixelSampler) instead of the host
+    optimizer: str = "adamw"            # "muon": the MLPs' weight matrices by Muon, everything else by AdamW
     own_heads_only: bool = True         # training renders each modality's rays through its own head only
 
 
@@ -465,6 +526,14 @@ def backward_batched(total: torch.Tensor, between=None, mid=None, cuts=None) -> 
         fx._WGRAD_DEFER[0] = None
         fx._WGRAD_DEFER_STREAM[0] = None
         fx.wn_bwd_flush()
+
+
+def muon_matrices(model: nn.Module) -> List[nn.Parameter]:
+    """The parameters that Muon steps: the MLPs' weight directions (weight norm's original1) and plain weights with at
+    least two rows and columns; tables, biases, norms and single rows stay with AdamW."""
+    return [p for name, p in model.named_parameters()
+            if p.dim() == 2 and min(p.shape) > 1 and (name.endswith("parametrizations.weight.original1") or
+                                                      name.endswith(".weight"))]
 
 
 class Trainer:
@@ -517,10 +586,16 @@ class Trainer:
         if cfg.gpu_sampler:
             from .data import GPUPixelSampler
             self.gpu_sampler = GPUPixelSampler(self.images, cfg.num_rays_per_modality, cfg.seed, rank)
-        self.fields = FlatGroup(list(self.model.parameters()), lr=1e-3, weight_decay=0.01, eps=1e-15)
+        if cfg.optimizer not in ("adamw", "muon"):
+            raise ValueError(f"optimizer must be 'adamw' or 'muon', got {cfg.optimizer!r}")
+        mats = muon_matrices(self.model) if cfg.optimizer == "muon" else []
+        rest = [p for p in self.model.parameters() if not any(p is q for q in mats)]
+        self.fields = FlatGroup(rest, lr=1e-3, weight_decay=0.01, eps=1e-15)
+        self.matrices = MuonGroup(mats, lr=1e-3, weight_decay=0.01) if mats else None
         pose_params = list(self.pose.parameters())
         self.poses = FlatGroup(pose_params, lr=1e-4, weight_decay=0.01, eps=1e-15) if pose_params else None
-        self.optim = OptimBank([self.fields, self.poses]) if self.fields.flat.device.type == "cuda" else None
+        self.groups = [g for g in (self.fields, self.matrices, self.poses) if g is not None]
+        self.optim = OptimBank(self.groups) if self.fields.flat.device.type == "cuda" else None
         self.step = 0
 
     def targets_for(self, coords: Dict[str, torch.Tensor], sel: Dict[str, torch.Tensor]):
@@ -546,9 +621,8 @@ class Trainer:
         volume_rendering.py:227-230) are applied for the current step first, as the reference's trainer does."""
         losses, total, outputs = self.compute_grads(coords, targets, rng, ddp)
         f = lr_factor(self.step, self.cfg.max_iters)
-        self.fields.step(f)
-        if self.poses is not None:
-            self.poses.step(f)
+        for g in self.groups:
+            g.step(f)
         self.step += 1
         return losses, total, outputs
 
@@ -580,10 +654,9 @@ class Trainer:
                 band = self.masks[m][coords_d[m][:, 1].long(), coords_d[m][:, 2].long()].long()[:, None]
                 outputs[m][m] = select_right_channel(outputs[m][m], band)
         losses, total = compute_loss(outputs, targets_d, self.modalities, self.step, max_iters=self.cfg.max_iters)
-        self.fields.zero_grad()
-        if self.poses is not None:
-            self.poses.zero_grad()
-        groups = [self.fields] + ([self.poses] if self.poses is not None else [])
+        groups = self.groups
+        for g in groups:
+            g.zero_grad()
         if ddp is not None and ddp.world > 1:
             # hash-table gradients are all-reduced as soon as their backward kernels are queued (overlapping the rest
             # of the backward), everything else after it

@@ -8,6 +8,7 @@ on the HIP kernels of libmms_hip.so (functions.py); nothing here has a CPU path.
 
   HashEncoding(config, in_dim)                    encodings.py:184-310   forward(x_hat [...,3]) -> [..., L F]
   NeRFEncoding(config, in_dim)                    encodings.py:131-182   forward(x [...,3])
+  EmbeddingEncoding(config, in_dim)               not in the reference: learned codes of an index, forward(i [...,1])
   FeatureGrid(config, input_dim, output_dim)      feature_structures.py:56-127
   FeatureGridAndMLP(config, input_dim, output_dim) feature_structures.py:130-173
   SDFField(config)                                surface_field.py:80-116  forward(x) -> (sdf, geo), single_output
@@ -30,7 +31,7 @@ from . import _lib
 from . import functions as fx
 from . import model as mm
 from . import pipeline as pl
-from .hip_ops import HashGridFunction
+from .hip_ops import EmbeddingFunction, HashGridFunction
 
 
 # ------------------------------------------------------------------------------------------------
@@ -71,6 +72,21 @@ class NeRFEncodingConfig(_Setup):
     @property
     def _target(self):
         return NeRFEncoding
+
+
+@dataclass
+class EmbeddingEncodingConfig(_Setup):
+    """A learned table of codes (per training view, per camera): ``scale`` multiplies the codes, ``init_scale`` their
+    normal initial values; ``padding_index`` (optional) starts at zero and gets no gradient."""
+    num_embeddings: int = 64
+    embedding_dim: int = 32
+    scale: float = 1.0
+    init_scale: float = 0.01
+    padding_index: Optional[int] = None
+
+    @property
+    def _target(self):
+        return EmbeddingEncoding
 
 
 @dataclass
@@ -284,6 +300,35 @@ class NeRFEncoding(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         shp = x.shape[:-1]
         return _NeRFEncodingFunction.apply(x.reshape(-1, 3), self.F).reshape(*shp, self.get_out_dim())
+
+
+class EmbeddingEncoding(nn.Module):
+    """Learned codes of an integer index, in the encodings' interface: forward(i [..., 1] int32 or int64) ->
+    scale * table[i] [..., embedding_dim] (an index outside the table: zeros).  RayBundle.camera_indices are such
+    indices: the codes of the training views go into RadianceField's additional inputs.  Parameter ``table``
+    [num_embeddings, embedding_dim]; its gradient has the same bits on each run (hip_ops.embedding_backward)."""
+
+    def __init__(self, config, in_dim: int = 1):
+        super().__init__()
+        rows, dim, pad = int(config.num_embeddings), int(config.embedding_dim), config.padding_index
+        if in_dim != 1:
+            raise ValueError("EmbeddingEncoding takes one index")
+        if rows < 1 or dim < 1 or (pad is not None and not -rows <= pad < rows):
+            raise ValueError(f"EmbeddingEncoding: {rows} codes of {dim} values, padding_index {pad}")
+        self.config, self.input_dim = config, in_dim
+        self.padding_index = None if pad is None else pad % rows
+        table = torch.randn(rows, dim) * float(config.init_scale)
+        if pad is not None:
+            table[pad] = 0.0
+        self.table = nn.Parameter(table)
+
+    def get_out_dim(self) -> int:
+        return self.table.shape[1]
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dim() == 0 or x.shape[-1] != self.input_dim:
+            raise ValueError(f"EmbeddingEncoding: indices must be [..., 1], got {tuple(x.shape)}")
+        return EmbeddingFunction.apply(x[..., 0], self.table, float(self.config.scale), self.padding_index)
 
 
 class FeatureGrid(mm.FeatureGrid):
