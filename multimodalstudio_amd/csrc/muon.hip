@@ -27,17 +27,27 @@
 #include "common.h"
 #include "chain_common.h"
 
+#include <algorithm>
+
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+// pointers read from a table are generic to the compiler (flat loads and stores): these are to device memory
+#define MMS_GLOBAL __attribute__((address_space(1)))
+typedef MMS_GLOBAL char gchar;
+typedef MMS_GLOBAL _Float16 ghalf;
+typedef MMS_GLOBAL half4 ghalf4;
+typedef MMS_GLOBAL half8 ghalf8;
 
+constexpr int kMaxMatrices = 4096;       // (or stacks) per call
 constexpr int kNsItems = 48;             // matrices (or stacks of them) per launch: the argument struct stays < 4 KB
 constexpr float kScale = 1024.f;         // fp16 operands hold 2^10 times their value
 constexpr float kDescale = 1.f / 1024.f; // a product of two of them, back to 2^10 times its value
 constexpr int kNormBlocks = 1024;        // blocks per matrix that sum squares, at most
 constexpr int kNormElems = 8192;         // elements per such block, at least
+constexpr int64_t kMaxBlocks = 1 << 23;  // of a launch (times its threads: below 2^32)
 
 struct NsItem {
   const void* g;       // gradient (or the matrix to orthogonalise)
@@ -56,6 +66,19 @@ struct NsArgs {
   NsItem it[kNsItems];
 };
 
+// The items again, in the workspace: written by the first launch, read by the others.  (Kernel arguments lie in host
+// memory: 3.6 KB of them cost each launch several us on the host, and each block a slow read.)
+struct NsTable {
+  int blk0[4][64];          // first block of each item: packing, A, B, X; INT_MAX past the last
+  NsItem it[kNsItems];
+};
+constexpr int64_t kTableBytes = 4608;
+static_assert(sizeof(NsTable) <= kTableBytes, "the table's part of the workspace");
+enum { MAP_PACK = 0, MAP_A = 1, MAP_B = 2, MAP_X = 3 };
+struct NsTiles {
+  int a, b, x;
+};
+
 struct NsStep {
   float momentum, rest;     // mu and 1 - mu, each rounded once (1 - 0.95f is 2e-7 off)
   int nesterov;
@@ -70,10 +93,10 @@ struct NsStep {
 // k, so that a 128-byte line holds both), 1 with hi only.
 struct NsLayout {
   int rp, cp, w;
-  __host__ __device__ NsLayout(int rows, int cols, int tile, int w_) : w(w_) {
+  __host__ __device__ NsLayout(int rows, int cols, int w_) : w(w_) {
     const int r = rows < cols ? rows : cols, c = rows < cols ? cols : rows;
-    rp = (r + tile - 1) / tile * tile;
-    cp = (c + tile - 1) / tile * tile;
+    rp = (r + 63) / 64 * 64;
+    cp = (c + 63) / 64 * 64;
   }
   __host__ __device__ int64_t x() const { return kNormBlocks * (int64_t)sizeof(double); }
   __host__ __device__ int64_t xt(int i) const { return x() + (int64_t)rp * cp * w * 2 * (1 + i); }
@@ -83,25 +106,54 @@ struct NsLayout {
   __host__ __device__ int64_t bytes() const { return xlo() + (w == 1 ? (int64_t)rp * cp * 2 : 0); }
 };
 
+// the item of a block: every lane compares one item's first block (one load; a search through the arguments, which lie
+// in host memory, waits for each of its steps)
 __device__ __forceinline__ int find_item(const NsArgs& A, int blk) {
-  int lo = 0, hi = A.n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (A.blk0[mid] <= blk) lo = mid; else hi = mid;
-  }
-  return lo;
+  const int lane = threadIdx.x & 63;
+  const bool before = lane < A.n && A.blk0[lane < kNsItems ? lane : 0] <= blk;
+  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(before)) - 1);
+}
+__device__ __forceinline__ int find_item(const NsTable* T, int map, int blk, int& first) {
+  const int b0 = T->blk0[map][threadIdx.x & 63];
+  const int i = __builtin_amdgcn_readfirstlane(__popcll(__ballot(b0 <= blk)) - 1);
+  first = __builtin_amdgcn_readlane(b0, i);
+  return i;
+}
+// the item by scalar loads (nothing writes the table while this launch runs)
+__device__ __forceinline__ NsItem load_item(const NsTable* T, int i) {
+  typedef const __attribute__((address_space(4))) uint64_t* words;
+  const words src = (words)(uintptr_t)(T->it + i);
+  static_assert(sizeof(NsItem) % 8 == 0, "whole words");
+  uint64_t w[sizeof(NsItem) / 8];
+#pragma unroll
+  for (size_t q = 0; q < sizeof(NsItem) / 8; ++q) w[q] = src[q];
+  return __builtin_bit_cast(NsItem, w);
 }
 
-__device__ __forceinline__ float load1(const void* p, int64_t i, bool bf16) {
-  if (bf16) return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
-  return ((const float*)p)[i];
+// blocks of a matrix in each launch
+__host__ __device__ inline int norm_blocks(int64_t rows, int64_t cols) {
+  const int64_t nb = (rows * cols + kNormElems - 1) / kNormElems;
+  return nb < 1 ? 1 : nb > kNormBlocks ? kNormBlocks : (int)nb;
+}
+__host__ __device__ inline int pack_blocks(const NsLayout& L) { return (L.rp / 64) * (L.cp / 64); }
+__host__ __device__ inline int gram_blocks(const NsLayout& L, int tile) {
+  const int n = (L.rp + tile - 1) / tile;
+  return n * (n + 1) / 2;
+}
+__host__ __device__ inline int full_blocks(const NsLayout& L, int tile) {
+  return ((L.rp + tile - 1) / tile) * ((L.cp + tile - 1) / tile);
+}
+
+__device__ __forceinline__ float load1(const MMS_GLOBAL void* p, int64_t i, bool bf16) {
+  if (bf16) return __uint_as_float((uint32_t)((const MMS_GLOBAL uint16_t*)p)[i] << 16);
+  return ((const MMS_GLOBAL float*)p)[i];
 }
 __device__ __forceinline__ uint16_t to_bf16(float x) {
   return __builtin_bit_cast(uint16_t, (__bf16)x);
 }
-__device__ __forceinline__ void store1(void* p, int64_t i, bool bf16, float v) {
-  if (bf16) ((uint16_t*)p)[i] = to_bf16(v);
-  else ((float*)p)[i] = v;
+__device__ __forceinline__ void store1(MMS_GLOBAL void* p, int64_t i, bool bf16, float v) {
+  if (bf16) ((MMS_GLOBAL uint16_t*)p)[i] = to_bf16(v);
+  else ((MMS_GLOBAL float*)p)[i] = v;
 }
 
 __device__ __forceinline__ float clip_of(const NsStep& s) {
@@ -113,16 +165,33 @@ __device__ __forceinline__ float clip_of(const NsStep& s) {
 // ---- momentum and the sum of squares ----------------------------------------------------------------------------
 // Reads g and m, writes m (12 bytes an element in fp32), and leaves each block's sum of u^2, in double: gradients of
 // 1e-25 or 1e25 keep their norm.  u is not stored: the next launch forms it again from the g and m it has to read.
-__global__ __launch_bounds__(256) void muon_momentum_kernel(NsArgs A, NsStep S, int bf16, int tile, int w) {
+__global__ __launch_bounds__(256) void muon_momentum_kernel(NsArgs A, NsStep S, int bf16, int w, NsTiles tiles,
+                                                            NsTable* __restrict__ table) {
   __shared__ double red[4];
+  if (blockIdx.x == 0 && threadIdx.x < 64) {
+    const int i = threadIdx.x, k = i < A.n ? i : 0;
+    const NsItem it = A.it[k];
+    const NsLayout L(it.rows, it.cols, w);
+    const int count[4] = {pack_blocks(L) * it.batch, gram_blocks(L, tiles.a) * it.batch, gram_blocks(L, tiles.b) * it.batch,
+                          full_blocks(L, tiles.x) * it.batch};
+    for (int q = 0; q < 4; ++q) {
+      int x = i < A.n ? count[q] : 0;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o);
+        if (i >= o) x += y;
+      }
+      table->blk0[q][i] = i < A.n ? x - count[q] : 0x7fffffff;
+    }
+    if (i < A.n) table->it[i] = it;
+  }
   const int ii = find_item(A, blockIdx.x);
   const NsItem it = A.it[ii];
-  const NsLayout L(it.rows, it.cols, tile, w);
+  const NsLayout L(it.rows, it.cols, w);
   const int per = (A.blk0[ii + 1] - A.blk0[ii]) / it.batch;
   const int k = (blockIdx.x - A.blk0[ii]) / per, b = (blockIdx.x - A.blk0[ii]) % per;
   const int64_t n = (int64_t)it.rows * it.cols;
-  const char* g = (const char*)it.g + k * it.bsg * (bf16 ? 2 : 4);
-  float* m = it.m ? it.m + k * n : nullptr;
+  const gchar* g = (const gchar*)it.g + k * it.bsg * (bf16 ? 2 : 4);
+  MMS_GLOBAL float* m = it.m ? (MMS_GLOBAL float*)it.m + k * n : nullptr;
   const float clip = clip_of(S), w1 = S.rest, mu = S.momentum;
   double sum = 0.0;
   const auto one = [&](int64_t i, float gi, float& mi) {
@@ -136,20 +205,20 @@ __global__ __launch_bounds__(256) void muon_momentum_kernel(NsArgs A, NsStep S, 
   };
   const bool dense = it.ldg == it.cols;
   const int64_t step = (int64_t)per * 256;
-  if (dense && n % 4 == 0 && ((uintptr_t)g & (bf16 ? 7 : 15)) == 0 && ((uintptr_t)m & 15) == 0) {
+  if (dense && n % 4 == 0 && ((uint64_t)g & (bf16 ? 7 : 15)) == 0 && ((uint64_t)m & 15) == 0) {
     for (int64_t i = (int64_t)b * 256 + threadIdx.x; i < n / 4; i += step) {
       float gi[4];
       if (bf16) {
-        const uint2 q = ((const uint2*)g)[i];
+        const uint2 q = *(const uint2*)((const char*)g + 8 * i);
         gi[0] = __uint_as_float(q.x << 16); gi[1] = __uint_as_float(q.x & 0xffff0000u);
         gi[2] = __uint_as_float(q.y << 16); gi[3] = __uint_as_float(q.y & 0xffff0000u);
       } else {
-        const float4 q = ((const float4*)g)[i];
+        const float4 q = *(const float4*)((const char*)g + 16 * i);
         gi[0] = q.x; gi[1] = q.y; gi[2] = q.z; gi[3] = q.w;
       }
-      float4 mi = m ? ((const float4*)m)[i] : float4{0.f, 0.f, 0.f, 0.f};
+      float4 mi = m ? *(const float4*)((const float*)m + 4 * i) : float4{0.f, 0.f, 0.f, 0.f};
       one(4 * i, gi[0], mi.x); one(4 * i + 1, gi[1], mi.y); one(4 * i + 2, gi[2], mi.z); one(4 * i + 3, gi[3], mi.w);
-      if (m) ((float4*)m)[i] = mi;
+      if (m) *(float4*)((float*)m + 4 * i) = mi;
     }
   } else {
     for (int64_t i = (int64_t)b * 256 + threadIdx.x; i < n; i += step) {
@@ -164,10 +233,12 @@ __global__ __launch_bounds__(256) void muon_momentum_kernel(NsArgs A, NsStep S, 
   if (threadIdx.x == 0) ((double*)(it.ws + k * L.bytes()))[b] = red[0] + red[1] + red[2] + red[3];
 }
 
-// position of (row, k) in an operand of K columns: with hi and lo, 32 of each in turn
+// Position of (row, k) in an operand of R rows: 32 columns at a time, all rows of them one after another, so that a
+// stage of a tile is one contiguous piece (rows of a power of two of bytes apart would meet in few of the L2's
+// channels).  With hi and lo, a row holds 32 of each.
 template <int W>
-__device__ __forceinline__ int64_t at(int64_t row, int64_t K, int k) {
-  return W == 1 ? row * K + k : row * K * 2 + (k >> 5) * 64 + (k & 31);
+__device__ __forceinline__ int64_t at(int row, int R, int k) {
+  return ((int64_t)(k >> 5) * R + row) * (32 * W) + (k & 31);
 }
 
 template <int N>
@@ -182,23 +253,22 @@ __device__ __forceinline__ void split_n(const float* v, _Float16* hi, _Float16* 
 // ---- X and X^T of u / |u| -----------------------------------------------------------------------------------------
 // One 64 x 64 tile of u per block through LDS, written in both orders; the rows and columns of the padding as zeros.
 template <int W>
-__global__ __launch_bounds__(256) void ns_pack_kernel(NsArgs A, NsStep S, int bf16, int tile) {
+__global__ __launch_bounds__(256) void ns_pack_kernel(const NsTable* __restrict__ T, NsStep S, int bf16) {
   __shared__ float t[64][65];
   __shared__ double red[4];
-  const int ii = find_item(A, blockIdx.x);
-  const NsItem it = A.it[ii];
-  const NsLayout L(it.rows, it.cols, tile, W);
+  int first;
+  const NsItem it = load_item(T, find_item(T, MAP_PACK, blockIdx.x, first));
+  const NsLayout L(it.rows, it.cols, W);
   const bool tall = it.rows > it.cols;
   const int tr = (tall ? L.cp : L.rp) / 64, tc = (tall ? L.rp : L.cp) / 64;
-  const int q = blockIdx.x - A.blk0[ii];
+  const int q = blockIdx.x - first;
   const int k = q / (tr * tc), i0 = (q / tc) % tr * 64, j0 = q % tc * 64;
-  char* ws = it.ws + k * L.bytes();
+  gchar* ws = (gchar*)it.ws + k * L.bytes();
   const int64_t n = (int64_t)it.rows * it.cols;
   // |u|: the partial sums in a fixed order
-  const int64_t nb64 = (n + kNormElems - 1) / kNormElems;
-  const int nb = nb64 < 1 ? 1 : nb64 > kNormBlocks ? kNormBlocks : (int)nb64;
+  const int nb = norm_blocks(it.rows, it.cols);
   double sum = 0.0;
-  for (int i = threadIdx.x; i < nb; i += 256) sum += ((const double*)ws)[i];
+  for (int i = threadIdx.x; i < nb; i += 256) sum += ((const MMS_GLOBAL double*)ws)[i];
   for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
   __syncthreads();
@@ -206,8 +276,8 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(NsArgs A, NsStep S, int bf
   norm = norm < S.eps ? S.eps : norm;
   const double inv = (double)kScale / norm;
 
-  const char* g = (const char*)it.g + k * it.bsg * (bf16 ? 2 : 4);
-  const float* m = it.m ? it.m + k * n : nullptr;
+  const gchar* g = (const gchar*)it.g + k * it.bsg * (bf16 ? 2 : 4);
+  const MMS_GLOBAL float* m = it.m ? (const MMS_GLOBAL float*)it.m + k * n : nullptr;
   const float clip = clip_of(S), mu = S.momentum;
   for (int e = threadIdx.x; e < 64 * 64; e += 256) {
     const int i = i0 + (e >> 6), j = j0 + (e & 63);
@@ -225,27 +295,27 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(NsArgs A, NsStep S, int bf
   }
   __syncthreads();
   // the tile in its own order is X (wide) or X^T (tall); the other one gets the transposed tile
-  _Float16* X = (_Float16*)(ws + L.x());
-  _Float16* XT = (_Float16*)(ws + L.xt(0));
-  _Float16* Xlo = (_Float16*)(ws + L.xlo());
-  _Float16* same = tall ? XT : X;
-  _Float16* other = tall ? X : XT;
-  const int64_t ks = tall ? L.rp : L.cp, ko = tall ? L.cp : L.rp;
+  ghalf* X = (ghalf*)(ws + L.x());
+  ghalf* XT = (ghalf*)(ws + L.xt(0));
+  ghalf* Xlo = (ghalf*)(ws + L.xlo());
+  ghalf* same = tall ? XT : X;
+  ghalf* other = tall ? X : XT;
+  const int rs = tall ? L.cp : L.rp, ro = tall ? L.rp : L.cp;
   for (int e = threadIdx.x; e < 64 * 16; e += 256) {
-    const int a = e >> 4, b = (e & 15) * 4;
+    const int a = (e >> 3) & 63, b = (e >> 9) * 32 + (e & 7) * 4;   // 8 threads: the 32 columns of a row; then rows
     half4 hi, lo;
     float v[4] = {t[a][b], t[a][b + 1], t[a][b + 2], t[a][b + 3]};
     split_n<4>(v, (_Float16*)&hi, (_Float16*)&lo);
-    _Float16* d = same + at<W>(i0 + a, ks, j0 + b);
-    *(half4*)d = hi;
-    if (W == 2) *(half4*)(d + 32) = lo;
-    else if (!tall) *(half4*)(Xlo + (i0 + a) * ks + j0 + b) = lo;
+    int64_t d = at<W>(i0 + a, rs, j0 + b);
+    *(ghalf4*)(same + d) = hi;
+    if (W == 2) *(ghalf4*)(same + d + 32) = lo;
+    else if (!tall) *(ghalf4*)(Xlo + d) = lo;
     float u[4] = {t[b][a], t[b + 1][a], t[b + 2][a], t[b + 3][a]};
     split_n<4>(u, (_Float16*)&hi, (_Float16*)&lo);
-    d = other + at<W>(j0 + a, ko, i0 + b);
-    *(half4*)d = hi;
-    if (W == 2) *(half4*)(d + 32) = lo;
-    else if (tall) *(half4*)(Xlo + (j0 + a) * ko + i0 + b) = lo;
+    d = at<W>(j0 + a, ro, i0 + b);
+    *(ghalf4*)(other + d) = hi;
+    if (W == 2) *(ghalf4*)(other + d + 32) = lo;
+    else if (tall) *(ghalf4*)(Xlo + d) = lo;
   }
 }
 
@@ -258,31 +328,39 @@ __device__ __forceinline__ void lds_dma16_s(const char* base, uint32_t off, uint
                : "memory", "m0");
 }
 
-// One TILE x TILE tile of P Q^T per block.  WM x WN: a wave's part.  A stage is 128 bytes of every row (64 values, or
-// 32 hi and 32 lo), brought to LDS by DMA; the 16-byte chunk c of row i lies at c ^ (i & 7), which makes the fragment
-// reads (8 lanes = 8 rows, one chunk) free of bank conflicts.  NBUF stages form a ring, NBUF - 1 of them in flight.
+// a pointer that every lane holds alike, in scalar registers
+__device__ __forceinline__ const char* uniform(const char* p) {
+  const uint64_t v = (uint64_t)(uintptr_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return (const char*)(uintptr_t)((uint64_t)hi << 32 | lo);
+}
+
+// One TILE x TILE tile of P Q^T per block.  WM x WN: a wave's part.  A stage is 128 bytes of every row (64 values, or 32
+// hi and 32 lo), brought to LDS by DMA; the 16-byte chunk c of row i lies at c ^ (i & 7), which makes the fragment reads
+// (8 lanes = 8 rows, one chunk) free of bank conflicts.  NBUF stages form a ring, NBUF - 1 of them in flight.
 template <int TILE, int WM, int WN, int NBUF, int W, int PHASE>
 __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_kernel(
-    NsArgs A, NsStep S, float ca, float cb, float cc, int parity, int bf16) {
+    const NsTable* __restrict__ T, NsStep S, float ca, float cb, float cc, int parity, int bf16) {
   constexpr int NWM = TILE / WM, NWN = TILE / WN, NW = NWM * NWN, NT = NW * 64;
   constexpr int STAGE = 2 * TILE * 128;          // bytes
-  constexpr int LOADS = STAGE / (NW * 1024);     // DMA instructions per wave and stage
+  constexpr int LOADS = STAGE / (NW * 1024);     // DMA instructions per wave and stage, 8 rows each
   constexpr int FM = WM / 16, FN = WN / 16;
   constexpr int SLAB = 64 * (TILE + 1) * 4;
   __shared__ __attribute__((aligned(1024))) char lds[NBUF * STAGE > SLAB ? NBUF * STAGE : SLAB];
 
-  // blocks b, b + 8, ... share an XCD: give each XCD a run of neighbouring tiles
-  int blk = blockIdx.x;
-  {
-    const int nblk = gridDim.x, per = nblk / 8, rest = nblk % 8, x = blk & 7;
-    blk = x * per + (x < rest ? x : rest) + (blk >> 3);
-  }
-  const int ii = find_item(A, blk);
-  const NsItem it = A.it[ii];
-  const NsLayout L(it.rows, it.cols, TILE, W);
-  const int nr = L.rp / TILE, nc = L.cp / TILE;
-  int q = blk - A.blk0[ii], ti, tj;
+  int first;
+  const NsItem it = load_item(T, find_item(T, PHASE == PHASE_A ? MAP_A : PHASE == PHASE_B ? MAP_B : MAP_X, blockIdx.x, first));
+  const NsLayout L(it.rows, it.cols, W);
+  const int nr = (L.rp + TILE - 1) / TILE, nc = (L.cp + TILE - 1) / TILE;
   const int per = PHASE <= PHASE_B ? nr * (nr + 1) / 2 : nr * nc;
+  int q = blockIdx.x - first, ti, tj;
+  {
+    // blocks b, b + 8, ... share an XCD: give each XCD a run of neighbouring tiles of the item
+    const int o = first & 7, x = (q + o) & 7, last = per * it.batch + o - 1;
+    int start = 0;
+    for (int y = 0; y < x; ++y) start += (last - y >= 0 ? ((last - y) >> 3) + 1 : 0) - (y < o ? 1 : 0);
+    q = start + ((q + o) >> 3) - (x < o ? 1 : 0);
+  }
   const int k = q / per;
   q -= k * per;
   if (PHASE <= PHASE_B) {
@@ -297,32 +375,41 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
     ti = grp * 4 + in % h;
     tj = in / h;
   }
-  char* ws = it.ws + k * L.bytes();
-  const _Float16* P = (const _Float16*)(ws + (PHASE == PHASE_A ? L.x() : PHASE == PHASE_B ? L.a() : L.b()));
-  const _Float16* Q = PHASE <= PHASE_B ? P : (const _Float16*)(ws + L.xt(parity));
+  gchar* ws = (gchar*)it.ws + k * L.bytes();
+  const ghalf* P = (const ghalf*)(ws + (PHASE == PHASE_A ? L.x() : PHASE == PHASE_B ? L.a() : L.b()));
+  const ghalf* Q = PHASE <= PHASE_B ? P : (const ghalf*)(ws + L.xt(parity));
   const int K = PHASE == PHASE_A ? L.cp : L.rp;
-  const int64_t ldb = (int64_t)K * W * 2;        // bytes between rows
-  const int stages = K * W / 64;
+  const int qrows = PHASE <= PHASE_B ? L.rp : L.cp;
+  const int stages = __builtin_amdgcn_readfirstlane(K * W / 64);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / NWN, wn = wave % NWN;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)lds;
-  // loads: instruction l of a wave brings rows 8 (l NW + wave) .. + 7 of [P tile; Q tile]
-  const char* pb = (const char*)P + (int64_t)ti * TILE * ldb;
-  const char* qb = (const char*)Q + (int64_t)tj * TILE * ldb;
-  uint32_t off[LOADS];
+  // Loads: an instruction brings 8 rows of a stage; the first half of them are P's, the others Q's.  (Its rows lie in one
+  // of the 64-row parts that operands are padded to: those past the operand are replaced by its tile's first ones, for
+  // results that nobody keeps.)
+  const char* src[LOADS];
 #pragma unroll
   for (int l = 0; l < LOADS; ++l) {
-    const int row = (8 * (l * NW + wave) + (lane >> 3)) % TILE;
-    off[l] = (uint32_t)(row * ldb) + (((lane & 7) ^ (lane >> 3)) << 4);
+    const int part = 8 * (l * NW + wave), row = part % TILE, row0 = (part < TILE ? ti : tj) * TILE;
+    const int left = (part < TILE ? L.rp : qrows) - row0;
+    src[l] = uniform((const char*)(part < TILE ? P : Q) + (int64_t)(row0 + (row < left ? row : 0)) * (64 * W));
   }
+  // the lane's chunk; in prec 1 a stage's row is two of the operand's 64-byte ones
+  const int lrow = lane >> 3, lchunk = (lane & 7) ^ lrow;
+  const uint32_t off = lrow * (64 * W) + (W == 1 ? lchunk & 3 : lchunk) * 16;
+  const uint32_t offp = off + (W == 1 ? (lchunk >> 2) * L.rp * 64 : 0);
+  const uint32_t offq = off + (W == 1 ? (lchunk >> 2) * qrows * 64 : 0);
   const auto issue = [&](int s) {
     const uint32_t dst = lds0 + (s % NBUF) * STAGE + wave * 1024;
+    const int64_t sp = (int64_t)s * L.rp * 128, sq = (int64_t)s * qrows * 128;
 #pragma unroll
-    for (int l = 0; l < LOADS; ++l)
-      lds_dma16_s((l * NW * 8 < TILE ? pb : qb) + (int64_t)s * 128, off[l], dst + l * NW * 1024);
+    for (int l = 0; l < LOADS; ++l) {
+      const bool p = 8 * (l * NW + wave) < TILE;
+      lds_dma16_s(src[l] + (p ? sp : sq), p ? offp : offq, dst + l * NW * 1024);
+    }
   };
-  static_assert((TILE / 8) % NW == 0, "an instruction loads rows of one operand for every wave");
+  static_assert(LOADS * NW * 8 == 2 * TILE, "whole instructions");
 
   floatx4 acc[FM][FN];
 #pragma unroll
@@ -330,8 +417,33 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  const int frow = lane & 15, fchunk = ((lane >> 4) ^ (lane & 7)) << 4;
+  // what the epilogue adds to the product: with 64-wide tiles, whose time is waiting, brought along with the operands
+  constexpr int OWN = TILE == 64 && PHASE != PHASE_A ? 64 * TILE / 4 / NT : 0;
+  half4 own_hi[OWN + 1], own_lo[OWN + 1];
+  // (the last product's results go to rows of the caller's: threads along the row; others as the operands lie: 8 threads
+  // for 32 columns, then the next row)
+  const auto place = [](int e, int& i, int& j) {
+    if (PHASE == PHASE_LAST) { i = e / (TILE / 4); j = e % (TILE / 4) * 4; }
+    else { i = (e >> 3) & 63; j = (e >> 9) * 32 + (e & 7) * 4; }
+  };
+  const auto own = [&](int i, int j, half4& hi, half4& lo) {
+    const int64_t d = at<W>(ti * TILE + i, L.rp, tj * TILE + j);
+    const ghalf* x = PHASE == PHASE_B ? P : (const ghalf*)(ws + L.x());
+    hi = *(const ghalf4*)(x + d);
+    if (W == 2) lo = *(const ghalf4*)(x + d + 32);
+    else if (PHASE >= PHASE_X) lo = *(const ghalf4*)((const ghalf*)(ws + L.xlo()) + d);
+    else lo = half4{0, 0, 0, 0};
+  };
+#pragma unroll
+  for (int o = 0; o < OWN; ++o) {
+    int i, j;
+    place(threadIdx.x + o * NT, i, j);
+    own(i, j, own_hi[o], own_lo[o]);
+  }
+
+  const int frow = lane & 15;
   for (int s = 0; s < NBUF - 1 && s < stages; ++s) issue(s);
+  const int fchunk = ((lane >> 4) ^ (lane & 7)) << 4;
   for (int s = 0; s < stages; ++s) {
     // stage s has arrived once only the loads issued after it are outstanding; all waves are then past stage s - 1
     if (s + NBUF - 2 < stages) wait_vm_barrier<(NBUF - 2) * LOADS>();
@@ -371,12 +483,12 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
   // epilogue: 64 rows at a time through LDS in fp32 (odd row length: columns are read without conflicts too)
   constexpr int LD = TILE + 1;
   float* slab = (float*)lds;
-  _Float16* X = (_Float16*)(ws + L.x());
-  _Float16* XT = (_Float16*)(ws + L.xt(parity ^ 1));
-  _Float16* Xlo = (_Float16*)(ws + L.xlo());
-  _Float16* D = (_Float16*)(ws + (PHASE == PHASE_A ? L.a() : L.b()));
+  ghalf* X = (ghalf*)(ws + L.x());
+  ghalf* XT = (ghalf*)(ws + L.xt(parity ^ 1));
+  ghalf* Xlo = (ghalf*)(ws + L.xlo());
+  ghalf* D = (ghalf*)(ws + (PHASE == PHASE_A ? L.a() : L.b()));
   const bool tall = it.rows > it.cols;
-  char* out = PHASE == PHASE_LAST ? (char*)it.p + k * it.bsp * (bf16 ? 2 : 4) : nullptr;
+  gchar* out = PHASE == PHASE_LAST ? (gchar*)it.p + k * it.bsp * (bf16 ? 2 : 4) : nullptr;
   const float decay = PHASE == PHASE_LAST && it.m ? (S.hyper ? S.hyper[0] : S.decay) : 0.f;
   const float gain = PHASE == PHASE_LAST ? (it.m ? (S.hyper ? S.hyper[1] : S.neg_lr) * it.scale : 1.f) * kDescale : 0.f;
   const auto put = [&](int row, int col, float v) {   // row, col of the caller's matrix
@@ -385,7 +497,9 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
     if (it.m) v = __builtin_fmaf(load1(out, e, bf16), decay, v);
     store1(out, e, bf16, v);
   };
+  const int width = PHASE <= PHASE_B ? L.rp : L.cp;
   for (int s = 0; s < TILE / 64; ++s) {
+    if (ti * TILE + s * 64 >= L.rp) break;
     if (s) __syncthreads();
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
@@ -400,24 +514,23 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
     }
     __syncthreads();
     const int i0 = ti * TILE + s * 64, j0 = tj * TILE;
-    for (int e = threadIdx.x; e < 64 * TILE / 4; e += NT) {
-      const int i = e / (TILE / 4), j = e % (TILE / 4) * 4;
+#pragma unroll
+    for (int o = 0; o < 64 * TILE / 4 / NT; ++o) {
+      int i, j;
+      place(threadIdx.x + o * NT, i, j);
+      if (TILE > 64 && j0 + j >= width) continue;
       float v[4];
 #pragma unroll
       for (int z = 0; z < 4; ++z) v[z] = slab[i * LD + j + z];
       half4 hi, lo;
-      if (PHASE == PHASE_B) {
-        const _Float16* d = P + at<W>(i0 + i, K, j0 + j);
-        hi = *(const half4*)d;
-        if (W == 2) lo = *(const half4*)(d + 32);
+      if (PHASE != PHASE_A) {
+        if (OWN) { hi = own_hi[OWN ? o : 0]; lo = own_lo[OWN ? o : 0]; }
+        else own(s * 64 + i, j, hi, lo);
 #pragma unroll
-        for (int z = 0; z < 4; ++z) v[z] = __builtin_fmaf(cb, W == 2 ? (float)hi[z] + (float)lo[z] : (float)hi[z], cc * v[z]);
-      } else if (PHASE >= PHASE_X) {
-        _Float16* d = X + at<W>(i0 + i, L.cp, j0 + j);
-        hi = *(const half4*)d;
-        lo = *(const half4*)(W == 2 ? d + 32 : Xlo + (int64_t)(i0 + i) * L.cp + j0 + j);
-#pragma unroll
-        for (int z = 0; z < 4; ++z) v[z] = __builtin_fmaf(ca, (float)hi[z] + (float)lo[z], v[z]);
+        for (int z = 0; z < 4; ++z) {
+          const float y = (float)hi[z] + (float)lo[z];
+          v[z] = PHASE == PHASE_B ? __builtin_fmaf(cb, y, cc * v[z]) : __builtin_fmaf(ca, y, v[z]);
+        }
       }
       if (PHASE != PHASE_A) {
 #pragma unroll
@@ -431,10 +544,11 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
         }
       } else {
         split_n<4>(v, (_Float16*)&hi, (_Float16*)&lo);
-        _Float16* d = PHASE == PHASE_X ? X + at<W>(i0 + i, L.cp, j0 + j) : D + at<W>(i0 + i, L.rp, j0 + j);
-        *(half4*)d = hi;
-        if (W == 2) *(half4*)(d + 32) = lo;
-        else if (PHASE == PHASE_X) *(half4*)(Xlo + (int64_t)(i0 + i) * L.cp + j0 + j) = lo;
+        const int64_t d = at<W>(i0 + i, L.rp, j0 + j);
+        ghalf* to = PHASE == PHASE_X ? X : D;
+        *(ghalf4*)(to + d) = hi;
+        if (W == 2) *(ghalf4*)(to + d + 32) = lo;
+        else if (PHASE == PHASE_X) *(ghalf4*)(Xlo + d) = lo;
       }
     }
     // the other order: X^T, the mirrored triangle, or a tall result
@@ -442,7 +556,10 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
     if (PHASE == PHASE_LAST && !tall) continue;
     __syncthreads();
     for (int e = threadIdx.x; e < 64 * TILE / 8; e += NT) {
-      const int j = e >> 3, i = (e & 7) * 8;
+      // operands: 4 threads for a row's 32 columns, then the next row; a result: 8 threads along the caller's row
+      const int f = PHASE == PHASE_LAST ? e >> 3 : e >> 2, j = f % TILE;
+      const int i = PHASE == PHASE_LAST ? (e & 7) * 8 : f / TILE * 32 + (e & 3) * 8;
+      if (TILE > 64 && j0 + j >= width) continue;
       float v[8];
 #pragma unroll
       for (int z = 0; z < 8; ++z) v[z] = slab[(i + z) * LD + j];
@@ -455,62 +572,93 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
       } else {
         half8 hi, lo;
         split_n<8>(v, (_Float16*)&hi, (_Float16*)&lo);
-        _Float16* d = (PHASE == PHASE_X ? XT : D) + at<W>(j0 + j, L.rp, i0 + i);
-        *(half8*)d = hi;
-        if (W == 2) *(half8*)(d + 32) = lo;
+        ghalf* d = (PHASE == PHASE_X ? XT : D) + at<W>(j0 + j, width, i0 + i);
+        *(ghalf8*)d = hi;
+        if (W == 2) *(ghalf8*)(d + 32) = lo;
       }
     }
   }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
-struct NsPlan {
-  int tile, w;
+// Operands of hi and lo: prec 0, and matrices whose results have too few entries for the roundings to average out.
+int width_of(int64_t rows, int64_t cols, int prec) { return prec == 0 || rows <= 128 || cols <= 128 ? 2 : 1; }
+
+// The launches of the matrices that share one table
+struct NsGroup {
+  NsArgs A;
+  int64_t norm, pack, a, b, x;   // blocks
+  NsTiles tiles;
 };
 
-// Tile and operand width of each matrix.  A large tile reads its operands fewer times but there are fewer of them: a
-// size is taken by the matrices that do not leave half a tile empty, if together they have a block for 3 of 4 CUs.
-void ns_plan(int n, const int64_t* batch, const int64_t* rows, const int64_t* cols, int prec, NsPlan* plan) {
-  for (int i = 0; i < n; ++i) plan[i].tile = 0;
-  for (int t = 256; t >= 64; t /= 2) {
-    int64_t blocks = 0;
-    const auto fits = [&](int i) {
-      const int64_t r = rows[i] < cols[i] ? rows[i] : cols[i];
-      return plan[i].tile == 0 && (t == 64 || r > t / 2);
-    };
-    for (int i = 0; i < n; ++i)
-      if (fits(i)) blocks += batch[i] * ((rows[i] + t - 1) / t) * ((cols[i] + t - 1) / t);
-    for (int i = 0; i < n; ++i)
-      if (fits(i) && (t == 64 || blocks >= 192)) plan[i] = NsPlan{t, t == 64 || prec == 0 ? 2 : 1};
+// The tile of a launch whose item i has `count(i, t)` tiles of `stages(i)` stages: the one whose last block should end
+// first.  Blocks start with the longest; a CU is busy for cost x (stages + 8) of each of its tiles (8: the epilogue), so
+// the end is neither before the n-th longest block had its turn on one of 256 CUs nor before the average CU is through.
+// Costs in us, from launches that fill the card: 64-wide tiles are bound by LDS reads, 128 by those and by products,
+// 192 and 256 by power (the clock falls to 1.6 GHz under 256-wide tiles, 1.2 PFLOP/s of fp16).  4096 x 4096, prec 1: A
+// 144, 109, 84, 104 us with 64, 128, 192, 256-wide tiles (253 of the 192-wide ones: one for each CU), X 229, 156, 178,
+// 136; six of 701 x 1100, prec 0: A 20, 28, 46, 70 us.
+constexpr int kTiles[4] = {256, 192, 128, 64};
+constexpr float kStageCost[2][4] = {{1.90f, 1.22f, 0.55f, 0.23f}, {2.25f, 1.40f, 0.78f, 0.26f}};
+template <typename Count, typename Stages>
+int choose_tile(int n, int w, const Count& count, const Stages& stages) {
+  int best = 64;
+  float least = 0.f;
+  for (int k = 0; k < 4; ++k) {
+    int64_t before = 0;
+    float sum = 0.f, end = 0.f;
+    for (int i = 0; i < n; ++i) {
+      const float each = kStageCost[w - 1][k] * (8 + stages(i));
+      const int64_t c = count(i, kTiles[k]);
+      before += c;
+      sum += each * c;
+      end = fmaxf(end, each * ((before + 255) / 256));
+    }
+    end = fmaxf(end, sum / 256);
+    if (k == 0 || end < least) { least = end; best = kTiles[k]; }
   }
+  return best;
 }
 
 int ns_check(const char* fn, int n, const int64_t* batch, const int64_t* rows, const int64_t* cols, int prec) {
-  MMS_REQUIRE(n >= 0 && n <= 4096, fn, "0 to 4096 matrices");
+  MMS_REQUIRE(n >= 0 && n <= kMaxMatrices, fn, "0 to 4096 matrices");
   MMS_REQUIRE(n == 0 || (batch && rows && cols), fn, "null size table");
   MMS_REQUIRE(prec == 0 || prec == 1, fn, "prec 0 (split fp16) or 1 (fp16)");
   for (int i = 0; i < n; ++i)
     MMS_REQUIRE(batch[i] >= 0 && rows[i] >= 0 && cols[i] >= 0 && batch[i] <= (1 << 20) && rows[i] <= (1 << 20) &&
-                    cols[i] <= (1 << 20) && batch[i] * ((rows[i] + 63) / 64) * ((cols[i] + 63) / 64) <= (1 << 28),
-                fn, "matrix sizes up to 2^20 a side and 2^28 64 x 64 tiles");
+                    cols[i] <= (1 << 20) && batch[i] * ((rows[i] + 255) / 256) * ((cols[i] + 255) / 256) * 16 <= kMaxBlocks &&
+                    batch[i] * ((rows[i] * cols[i] + kNormElems - 1) / kNormElems) <= kMaxBlocks,
+                fn, "matrix sizes up to 2^20 a side and 2^23 64 x 64 tiles a stack");
   return 0;
 }
 
-template <int TILE, int WM, int WN, int NBUF, int W>
-void launch_products(const NsArgs& gram, const NsArgs& full, const NsStep& S, int steps, float a, float b, float c,
-                     int bf16, hipStream_t s) {
-  constexpr int NT = (TILE / WM) * (TILE / WN) * 64;
+template <int W, int PHASE>
+void launch_product(int tile, const NsTable* T, int64_t blocks, const NsStep& S, float a, float b, float c, int parity,
+                    int bf16, hipStream_t s) {
+  const dim3 grid((unsigned)blocks);
+#define NS_LAUNCH(TILE, WM, WN, NBUF)                                                                            \
+  hipLaunchKernelGGL((ns_product_kernel<TILE, WM, WN, NBUF, W, PHASE>), grid, dim3((TILE / WM) * (TILE / WN) * 64), 0, \
+                     s, T, S, a, b, c, parity, bf16)
+  // 16 waves a CU where registers and LDS allow it: 8-wave blocks of 128 two at a time (482 us against 494 with 4 waves,
+  // X of muon's four 2048 x 2048 and two 2048 x 5632 in prec 0), 16 of 64 x 64 rather than 8 of 128 x 64 for 256 (483,
+  // 509), 4-wave blocks of 64 three at a time
+  if (tile == 64) NS_LAUNCH(64, 32, 32, 3);
+  else if (tile == 128) NS_LAUNCH(128, 64, 32, 2);
+  else if (tile == 192) NS_LAUNCH(192, 64, 48, 3);
+  else NS_LAUNCH(256, 64, 64, 2);
+#undef NS_LAUNCH
+}
+
+template <int W>
+void launch_group(const NsGroup& G, NsTable* T, const NsStep& S, int steps, float a, float b, float c, int bf16,
+                  hipStream_t s) {
+  hipLaunchKernelGGL(muon_momentum_kernel, dim3((unsigned)G.norm), dim3(256), 0, s, G.A, S, bf16, W, G.tiles, T);
+  hipLaunchKernelGGL((ns_pack_kernel<W>), dim3((unsigned)G.pack), dim3(256), 0, s, T, S, bf16);
   for (int i = 0; i < steps; ++i) {
-    hipLaunchKernelGGL((ns_product_kernel<TILE, WM, WN, NBUF, W, PHASE_A>), dim3(gram.blk0[gram.n]), dim3(NT), 0, s,
-                       gram, S, a, b, c, i & 1, bf16);
-    hipLaunchKernelGGL((ns_product_kernel<TILE, WM, WN, NBUF, W, PHASE_B>), dim3(gram.blk0[gram.n]), dim3(NT), 0, s,
-                       gram, S, a, b, c, i & 1, bf16);
-    if (i + 1 < steps)
-      hipLaunchKernelGGL((ns_product_kernel<TILE, WM, WN, NBUF, W, PHASE_X>), dim3(full.blk0[full.n]), dim3(NT), 0, s,
-                         full, S, a, b, c, i & 1, bf16);
-    else
-      hipLaunchKernelGGL((ns_product_kernel<TILE, WM, WN, NBUF, W, PHASE_LAST>), dim3(full.blk0[full.n]), dim3(NT), 0,
-                         s, full, S, a, b, c, i & 1, bf16);
+    launch_product<W, PHASE_A>(G.tiles.a, T, G.a, S, a, b, c, i & 1, bf16, s);
+    launch_product<W, PHASE_B>(G.tiles.b, T, G.b, S, a, b, c, i & 1, bf16, s);
+    if (i + 1 < steps) launch_product<W, PHASE_X>(G.tiles.x, T, G.x, S, a, b, c, i & 1, bf16, s);
+    else launch_product<W, PHASE_LAST>(G.tiles.x, T, G.x, S, a, b, c, i & 1, bf16, s);
   }
 }
 
@@ -536,43 +684,50 @@ int ns_run(const char* fn, int n, const int64_t* batch, const int64_t* rows, con
               "workspace too small (mms_muon_workspace) or not 256-byte aligned");
   hipStream_t s = mms::as_stream(stream);
   char* next = (char*)ws;
-  static thread_local NsPlan plan[4096];
-  ns_plan(n, batch, rows, cols, prec, plan);
-  for (int tile = 256; tile >= 64; tile /= 2) {
-    for (int first = 0; first < n;) {
-      // the next matrices of this tile that one launch holds
-      NsArgs sq{}, pack{}, gram{}, full{};
-      int64_t end[4] = {0, 0, 0, 0};
-      int w = 0, i = first;
-      for (; i < n && sq.n < kNsItems; ++i) {
-        if (plan[i].tile != tile || batch[i] * rows[i] * cols[i] == 0) continue;
-        w = plan[i].w;
-        const NsLayout L((int)rows[i], (int)cols[i], tile, w);
-        const int64_t nb = mms::grid_for(rows[i] * cols[i], kNormElems, kNormBlocks), nr = L.rp / tile, nc = L.cp / tile;
-        const int64_t add[4] = {batch[i] * nb, batch[i] * (L.rp / 64) * (L.cp / 64), batch[i] * (nr * (nr + 1) / 2),
-                                batch[i] * nr * nc};
-        if (sq.n && (end[1] + add[1] > (1LL << 30) || end[0] + add[0] > (1LL << 30))) break;
-        const NsItem it{g[i], m ? m[i] : nullptr, p[i], next, bsg[i], bsp[i], (int)ldg[i], (int)ldp[i], (int)rows[i],
-                        (int)cols[i], (int)batch[i], scale ? scale[i] : 1.f};
+  // largest first: their blocks are started first
+  static thread_local int order[kMaxMatrices];
+  int live = 0;
+  for (int i = 0; i < n; ++i)
+    if (batch[i] * rows[i] * cols[i] > 0) order[live++] = i;
+  std::sort(order, order + live, [&](int i, int j) {
+    const int64_t x = rows[i] + cols[i], y = rows[j] + cols[j];
+    return x != y ? x > y : i < j;
+  });
+  for (int w = 1; w <= 2; ++w) {
+    for (int at = 0; at < live;) {
+      // the next matrices that one table holds
+      NsGroup G{};
+      NsTable* T = (NsTable*)next;
+      for (; at < live && G.A.n < kNsItems; ++at) {
+        const int i = order[at];
+        if (width_of(rows[i], cols[i], prec) != w) continue;
+        const NsLayout L((int)rows[i], (int)cols[i], w);
+        const int64_t norm = batch[i] * norm_blocks(rows[i], cols[i]), pack = batch[i] * pack_blocks(L);
+        if (G.A.n && (G.norm + norm > kMaxBlocks || G.pack + pack > kMaxBlocks)) break;
+        if (G.A.n == 0) next += kTableBytes;
+        G.A.it[G.A.n] = NsItem{g[i], m ? m[i] : nullptr, p[i], next, bsg[i], bsp[i], (int)ldg[i], (int)ldp[i],
+                               (int)rows[i], (int)cols[i], (int)batch[i], scale ? scale[i] : 1.f};
+        G.A.blk0[G.A.n++] = (int)G.norm;
         next += batch[i] * L.bytes();
-        int z = 0;
-        for (NsArgs* A : {&sq, &pack, &gram, &full}) {
-          A->it[A->n] = it;
-          A->blk0[A->n] = (int)end[z];
-          end[z] += add[z];
-          A->blk0[++A->n] = (int)end[z++];
-        }
+        G.norm += norm;
+        G.pack += pack;
       }
-      first = i;
-      if (sq.n == 0) continue;
-      hipLaunchKernelGGL(muon_momentum_kernel, dim3(sq.blk0[sq.n]), dim3(256), 0, s, sq, S, bf16, tile, w);
-      if (w == 2) hipLaunchKernelGGL((ns_pack_kernel<2>), dim3(pack.blk0[pack.n]), dim3(256), 0, s, pack, S, bf16, tile);
-      else hipLaunchKernelGGL((ns_pack_kernel<1>), dim3(pack.blk0[pack.n]), dim3(256), 0, s, pack, S, bf16, tile);
-      if (tile == 256 && w == 2) launch_products<256, 128, 64, 2, 2>(gram, full, S, steps, a, b, c, bf16, s);
-      else if (tile == 256) launch_products<256, 128, 64, 2, 1>(gram, full, S, steps, a, b, c, bf16, s);
-      else if (tile == 128 && w == 2) launch_products<128, 64, 64, 2, 2>(gram, full, S, steps, a, b, c, bf16, s);
-      else if (tile == 128) launch_products<128, 64, 64, 2, 1>(gram, full, S, steps, a, b, c, bf16, s);
-      else launch_products<64, 32, 32, 8, 2>(gram, full, S, steps, a, b, c, bf16, s);
+      if (G.A.n == 0) break;
+      G.A.blk0[G.A.n] = (int)G.norm;
+      const NsItem* it = G.A.it;
+      const auto layout = [&](int i) { return NsLayout(it[i].rows, it[i].cols, w); };
+      const auto gram = [&](int i, int t) { return (int64_t)gram_blocks(layout(i), t) * it[i].batch; };
+      const auto full = [&](int i, int t) { return (int64_t)full_blocks(layout(i), t) * it[i].batch; };
+      G.tiles.a = choose_tile(G.A.n, w, gram, [&](int i) { return layout(i).cp * w / 64; });
+      G.tiles.b = choose_tile(G.A.n, w, gram, [&](int i) { return layout(i).rp * w / 64; });
+      G.tiles.x = choose_tile(G.A.n, w, full, [&](int i) { return layout(i).rp * w / 64; });
+      for (int i = 0; i < G.A.n; ++i) {
+        G.a += gram(i, G.tiles.a);
+        G.b += gram(i, G.tiles.b);
+        G.x += full(i, G.tiles.x);
+      }
+      if (w == 1) launch_group<1>(G, T, S, steps, a, b, c, bf16, s);
+      else launch_group<2>(G, T, S, steps, a, b, c, bf16, s);
       const int e = mms::check_launch(fn);
       if (e) return e;
     }
@@ -588,12 +743,10 @@ MMS_EXPORT int mms_muon_workspace(int n, const int64_t* batch, const int64_t* ro
   MMS_REQUIRE(bytes != nullptr, fn, "null output");
   const int rc = ns_check(fn, n, batch, rows, cols, prec);
   if (rc) return rc;
-  static thread_local NsPlan plan[4096];
-  ns_plan(n, batch, rows, cols, prec, plan);
   *bytes = 0;
   for (int i = 0; i < n; ++i)
     if (batch[i] * rows[i] * cols[i] > 0)
-      *bytes += batch[i] * NsLayout((int)rows[i], (int)cols[i], plan[i].tile, plan[i].w).bytes();
+      *bytes += kTableBytes + batch[i] * NsLayout((int)rows[i], (int)cols[i], width_of(rows[i], cols[i], prec)).bytes();
   return 0;
 }
 

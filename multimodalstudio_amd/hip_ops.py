@@ -245,6 +245,9 @@ class _on_device:
 def _matrices(t: torch.Tensor, what: str, copy: bool):
     """(tensor, batch, rows, cols, leading dimension, distance of a stack's matrices) of [..., rows, cols]; a layout
     that the kernels do not read in place is copied if ``copy``, else refused."""
+    if t.dim() == 2 and t.is_contiguous():     # the common case, at a few hundred ns of host time
+        rows, cols = t.shape
+        return t, 1, rows, cols, cols, 0
     if t.dim() < 2:
         raise ValueError(f"{what} must have at least two dimensions, got shape {tuple(t.shape)}")
     rows, cols = t.shape[-2:]
@@ -274,10 +277,9 @@ class _MatrixTable:
     def __init__(self, mats):
         n = self.n = len(mats)
         I64, VP = ctypes.c_int64 * n, ctypes.c_void_p * n
-        self.keep = [m[0] for m in mats]
-        self.batch, self.rows, self.cols = (I64(*[m[i] for m in mats]) for i in (1, 2, 3))
-        self.ptr = VP(*[m[0].data_ptr() for m in mats])
-        self.ld, self.bs = I64(*[m[4] for m in mats]), I64(*[m[5] for m in mats])
+        self.keep, batch, rows, cols, ld, bs = zip(*mats)
+        self.batch, self.rows, self.cols, self.ld, self.bs = I64(*batch), I64(*rows), I64(*cols), I64(*ld), I64(*bs)
+        self.ptr = VP(*[t.data_ptr() for t in self.keep])
 
 
 def _muon_workspace(tab: _MatrixTable, prec: int, device) -> torch.Tensor:
@@ -288,11 +290,12 @@ def _muon_workspace(tab: _MatrixTable, prec: int, device) -> torch.Tensor:
 
 def _check_matrices(ts, what: str):
     _check_dev(*ts)
+    device = ts[0].device if ts else None
     for t in ts:
         if t.dtype not in _MATRIX_DTYPES:
             raise TypeError(f"{what} must be float32 or bfloat16, got {t.dtype}")
-        if t.device != ts[0].device:
-            raise ValueError(f"{what} must be on one device, got {ts[0].device} and {t.device}")
+        if t.device != device:
+            raise ValueError(f"{what} must be on one device, got {device} and {t.device}")
 
 
 def _prec_of(dtype, prec: Optional[int]) -> int:
@@ -355,17 +358,16 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
         return
     _check_matrices(params, "muon_step: weights")
     _check_dev(*grads, *momenta, sumsq, hyper)
+    device = params[0].device
     for p, g, m in zip(params, grads, momenta):
-        if g.shape != p.shape or m.shape != p.shape:
+        shape = p.shape
+        if g.shape != shape or m.shape != shape:
             raise ValueError(f"muon_step: weights {tuple(p.shape)}, gradient {tuple(g.shape)}, momentum "
                              f"{tuple(m.shape)} must have one shape")
         if g.dtype != p.dtype or m.dtype != torch.float32 or not m.is_contiguous():
             raise ValueError("muon_step: gradients have their weights' type, momenta are contiguous float32")
-        if g.device != p.device or m.device != p.device:
+        if g.device != device or m.device != device:
             raise ValueError("muon_step: weights, gradients and momenta must be on one device")
-    for what, ts in (("weights", params), ("momenta", momenta)):
-        if len({t.data_ptr() for t in ts if t.numel()}) < sum(1 for t in ts if t.numel()):
-            raise ValueError(f"muon_step: the same {what} twice")
     for t, k in ((sumsq, 1), (hyper, 2)):
         if t is not None and (t.dtype != torch.float32 or t.numel() < k or not t.is_contiguous()
                               or t.device != params[0].device):
@@ -377,9 +379,13 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
             continue
         pr = _prec_of(dtype, prec)
         with torch.no_grad(), _on_device(params[0]):
-            w = _MatrixTable([_matrices(params[i].detach(), "muon_step: weights", False) for i in pick])
-            g = _MatrixTable([_matrices(grads[i].detach(), "muon_step: gradient", True) for i in pick])
+            w = _MatrixTable([_matrices(params[i], "muon_step: weights", False) for i in pick])
+            g = _MatrixTable([_matrices(grads[i], "muon_step: gradient", True) for i in pick])
             m = (ctypes.c_void_p * w.n)(*[momenta[i].data_ptr() for i in pick])
+            for what, ptrs in (("weights", w.ptr), ("momenta", m)):
+                full = [q for q, b, r, c in zip(ptrs, w.batch, w.rows, w.cols) if b * r * c]
+                if len(set(full)) < len(full):
+                    raise ValueError(f"muon_step: the same {what} twice")
             scale = (ctypes.c_float * w.n)(*[muon_scale(w.rows[k], w.cols[k], adjust) for k in range(w.n)])
             ws = _muon_workspace(w, pr, params[0].device)
             _lib.call("mms_muon_step", w.n, w.batch, w.rows, w.cols, w.ptr, w.ld, w.bs, g.ptr, g.ld, g.bs, m, scale,
