@@ -7,16 +7,41 @@
 // that occurs in half of the positions is spread over as many runs -- and sums each run in fp32 in one walk.  Rows
 // that lie inside a run are finished there; the pieces of a row that crosses runs go to the workspace and a second
 // launch adds them in order.  Rows that do not occur are found by a search in the sorted list and written as zeros by
-// further blocks of the same launch, so nothing is written twice.
+// further blocks of the same launch, but for the first rows, which the sort's launches clear beside their few blocks.
 #include "common.h"
 
 namespace {
 
 typedef __bf16 bf16_t;
 
-template <typename T> struct Vec16 { static constexpr int N = 16 / sizeof(T); };
-
-template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
+// a thread's piece of a row: 16 bytes, at any element's address (the card reads and writes them unaligned)
+template <typename T> struct Piece {
+  static constexpr int N = 16 / sizeof(T);
+  T v[N];
+};
+// The first `count` of its values.  WHOLE: rows are whole pieces, without a branch that keeps loads from being issued
+// together (65536 x 2048 bf16 into 131072 rows: 163 us against 240).
+template <bool WHOLE, typename T>
+__device__ __forceinline__ Piece<T> load_piece(const T* p, int count) {
+  Piece<T> x;
+  if (WHOLE || count >= Piece<T>::N) {
+    __builtin_memcpy(&x, p, 16);
+  } else {
+#pragma unroll
+    for (int q = 0; q < Piece<T>::N; ++q) x.v[q] = q < count ? p[q] : (T)0.f;
+  }
+  return x;
+}
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void store_piece(T* p, const Piece<T>& x, int count) {
+  if (WHOLE || count >= Piece<T>::N) {
+    __builtin_memcpy(p, &x, 16);
+  } else {
+#pragma unroll
+    for (int q = 0; q < Piece<T>::N; ++q)
+      if (q < count) p[q] = x.v[q];
+  }
+}
 
 struct Ids {
   const void* p;
@@ -36,34 +61,70 @@ __device__ __forceinline__ uint32_t key_at(const Ids& I, int64_t i) {
 }
 
 // ---- lookup -------------------------------------------------------------------------------------------------------
-// `lanes` threads (a power of two, at most 256) per row segment of lanes * N elements; blockIdx.y: the segment.
-template <typename T, int N>
+// A team of `lanes` threads (a power of two, at most 256) per R rows' segments of lanes pieces; blockIdx.y: the segment.
+template <typename T, bool WHOLE, int R>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(Ids I, int64_t n, const T* __restrict__ table, int64_t ldt,
                                                             int dim, int lanes_log2, float scale, T* __restrict__ out,
                                                             int64_t ldo) {
+  constexpr int N = Piece<T>::N;
   const int lane = threadIdx.x & ((1 << lanes_log2) - 1), team = threadIdx.x >> lanes_log2;
-  const int64_t i = (int64_t)blockIdx.x * (256 >> lanes_log2) + team;
+  const int64_t i0 = ((int64_t)blockIdx.x * (256 >> lanes_log2) + team) * R;
   const int c = ((int)blockIdx.y << lanes_log2 | lane) * N;
-  if (i >= n || c >= dim) return;
-  const int64_t v = id_at(I, i);
-  Pack<T, N> x{};
-  if (v >= 0 && v < I.rows) {
-    x = *(const Pack<T, N>*)(table + v * ldt + c);
+  if (i0 >= n || c >= dim) return;
+  int64_t v[R];
+  Piece<T> x[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) v[r] = id_at(I, i0 + r < n ? i0 + r : n - 1);
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (v[r] >= 0 && v[r] < I.rows) x[r] = load_piece<WHOLE>(table + v[r] * ldt + c, dim - c);
+    else x[r] = Piece<T>{};
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (i0 + r >= n) break;
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-      float y = (float)x.v[q] * scale;
+      float y = (float)x[r].v[q] * scale;
       asm("" : "+v"(y));   // rounded to fp32 before fp16 (not v_fma_mixlo's one rounding): the bits of the same product in torch
-      x.v[q] = (T)y;
+      x[r].v[q] = (T)y;
     }
+    store_piece<WHOLE>(out + (i0 + r) * ldo + c, x[r], dim - c);
   }
-  *(Pack<T, N>*)(out + i * ldo + c) = x;
+}
+
+// ---- zeros in the shadow of the sort --------------------------------------------------------------------------------
+// The sort keeps a few dozen blocks busy; further blocks of its launches clear the table's first rows meanwhile (rows
+// that occur among those are written twice).
+struct Zeros {
+  char* p;              // the first byte to clear
+  int64_t rows;         // rows of `bytes` bytes, `ld` apart
+  int64_t bytes, ld;
+  int first;            // the launch's first block that clears
+};
+constexpr int64_t kZeroChunk = 1 << 16;   // bytes per such block
+
+__device__ __forceinline__ bool clear_rows(const Zeros& Z) {
+  if ((int)blockIdx.x < Z.first) return false;
+  const bool dense = Z.ld == Z.bytes;
+  const int64_t bytes = dense ? Z.rows * Z.bytes : Z.bytes, per = (bytes + 15) / 16, all = dense ? per : per * Z.rows;
+  const int64_t begin = ((int64_t)blockIdx.x - Z.first) * (kZeroChunk / 16);
+  const int64_t end = begin + kZeroChunk / 16 < all ? begin + kZeroChunk / 16 : all;
+  const uint4 zero{0, 0, 0, 0};
+  for (int64_t e = begin + threadIdx.x; e < end; e += blockDim.x) {
+    const int64_t r = dense ? 0 : e / per, c = (e - r * per) * 16;
+    char* p = Z.p + r * Z.ld + c;
+    if (c + 16 <= bytes) __builtin_memcpy(p, &zero, 16);
+    else
+      for (int64_t b = c; b < bytes; b += 2, p += 2) *(uint16_t*)p = 0;
+  }
+  return true;
 }
 
 // ---- stable sort of (row, position) pairs ---------------------------------------------------------------------------
 constexpr int kSortThreads = 1024, kSortWaves = 16;
 constexpr int kMaxBits = 10;                       // of a digit
-constexpr int kTileRounds = 4;                     // a block of the many-block sort takes 4096 pairs
-constexpr int kOneRounds = 12;                     // up to 12288 pairs are sorted by one block
+constexpr int kTileRounds = 2;                     // a block of the many-block sort takes 2048 pairs
+constexpr int kOneRounds = 4;                      // up to 4096 pairs are sorted by one block
 constexpr int kScanBlocks = 64;                    // more blocks than this: their counts are scanned by a launch
 
 struct SortShared {
@@ -130,7 +191,8 @@ __device__ __forceinline__ uint32_t waves_before(int bits, SortShared& S) {
 
 // n <= kOneRounds * 1024 pairs by one block, all digits
 __global__ __launch_bounds__(kSortThreads) void sort_one_kernel(Ids I, int n, int bits, int passes,
-                                                                uint2* __restrict__ out) {
+                                                                uint2* __restrict__ out, Zeros Z) {
+  if (clear_rows(Z)) return;
   __shared__ SortShared S;
   __shared__ uint2 buf[kOneRounds * kSortThreads];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -156,7 +218,11 @@ __global__ __launch_bounds__(kSortThreads) void sort_one_kernel(Ids I, int n, in
     const bool last = pass + 1 == passes;
 #pragma unroll
     for (int j = 0; j < kOneRounds; ++j)
-      if (live[j]) (last ? out : buf)[S.base[digit[j]] + S.cnt[wave][digit[j]] + rank[j]] = p[j];
+      if (live[j]) {
+        const uint32_t to = S.base[digit[j]] + S.cnt[wave][digit[j]] + rank[j];
+        if (last) out[to] = p[j];
+        else buf[to] = p[j];
+      }
     if (last) break;
     __syncthreads();
 #pragma unroll
@@ -166,9 +232,11 @@ __global__ __launch_bounds__(kSortThreads) void sort_one_kernel(Ids I, int n, in
   }
 }
 
-// counts[block][digit] of the block's 4096 pairs; in == null: the pairs are (key of ids[i], i)
+// counts[digit][block] of the block's 2048 pairs (rows of ld: whole uint4s); in == null: the pairs are (key of ids[i], i)
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Ids I, const uint2* __restrict__ in, int64_t n,
-                                                                  int bits, int shift, uint32_t* __restrict__ counts) {
+                                                                  int bits, int shift, uint32_t* __restrict__ counts,
+                                                                  int ld, Zeros Z) {
+  if (clear_rows(Z)) return;
   __shared__ uint32_t hist[1 << kMaxBits];
   if (threadIdx.x < (1u << bits)) hist[threadIdx.x] = 0;
   __syncthreads();
@@ -179,17 +247,17 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Ids I, const u
     if (i < n) atomicAdd(&hist[((in ? in[i].x : key_at(I, i)) >> shift) & ((1u << bits) - 1)], 1u);
   }
   __syncthreads();
-  if (threadIdx.x < (1u << bits)) counts[((int64_t)blockIdx.x << bits) + threadIdx.x] = hist[threadIdx.x];
+  if (threadIdx.x < (1u << bits)) counts[(int64_t)threadIdx.x * ld + blockIdx.x] = hist[threadIdx.x];
 }
 
-// counts[block][digit] -> pairs of that digit in the blocks before, totals[digit]: a block per digit
-__global__ __launch_bounds__(kSortThreads) void sort_scan_kernel(uint32_t* __restrict__ counts, int nblk, int bits,
+// counts[digit][block] -> pairs of that digit in the blocks before, totals[digit]: a block per digit
+__global__ __launch_bounds__(kSortThreads) void sort_scan_kernel(uint32_t* __restrict__ counts, int nblk, int ld,
                                                                  uint32_t* __restrict__ totals) {
   __shared__ SortShared S;
   uint32_t before = 0;
   for (int b0 = 0; b0 < nblk; b0 += kSortThreads) {
     const int b = b0 + threadIdx.x;
-    uint32_t* c = counts + ((int64_t)b << bits) + blockIdx.x;
+    uint32_t* c = counts + (int64_t)blockIdx.x * ld + b;
     const uint32_t v = b < nblk ? *c : 0;
     const uint32_t x = block_scan(v, S) + before;
     if (b < nblk) *c = x;
@@ -203,9 +271,10 @@ __global__ __launch_bounds__(kSortThreads) void sort_scan_kernel(uint32_t* __res
 
 __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Ids I, const uint2* __restrict__ in, int64_t n,
                                                                     int bits, int shift,
-                                                                    const uint32_t* __restrict__ counts,
+                                                                    const uint32_t* __restrict__ counts, int ld,
                                                                     const uint32_t* __restrict__ totals,
-                                                                    uint2* __restrict__ out) {
+                                                                    uint2* __restrict__ out, int nblk, Zeros Z) {
+  if (clear_rows(Z)) return;
   __shared__ SortShared S;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t i0 = (int64_t)blockIdx.x * kTileRounds * kSortThreads + wave * kTileRounds * 64 + lane;
@@ -219,18 +288,29 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Ids I, const
     p[j] = !live[j] ? uint2{0, 0} : in ? in[i] : uint2{key_at(I, i), (uint32_t)i};
     digit[j] = (p[j].x >> shift) & ((1u << bits) - 1);
   }
+  // the digit's counts of all blocks (at most kScanBlocks of them), or the scanned one
+  uint32_t total = 0, before = 0;
+  uint4 c[kScanBlocks / 4];
+  if (!totals && threadIdx.x < (1u << bits)) {
+#pragma unroll
+    for (int q = 0; q < kScanBlocks / 4; ++q)
+      c[q] = q * 4 < nblk ? *(const uint4*)(counts + (int64_t)threadIdx.x * ld + q * 4) : uint4{0, 0, 0, 0};
+  }
   rank_pairs<kTileRounds>(digit, live, kTileRounds, bits, rank, S);
   waves_before(bits, S);
-  uint32_t total = 0, before = 0;
   if (threadIdx.x < (1u << bits)) {
     if (totals) {
       total = totals[threadIdx.x];
-      before = counts[((int64_t)blockIdx.x << bits) + threadIdx.x];
+      before = counts[(int64_t)threadIdx.x * ld + blockIdx.x];
     } else {
-      for (int b = 0; b < (int)gridDim.x; ++b) {
-        const uint32_t c = counts[((int64_t)b << bits) + threadIdx.x];
-        if (b < (int)blockIdx.x) before += c;
-        total += c;
+      const int n = nblk, me = blockIdx.x;
+      const auto add = [&](int b, uint32_t v) {
+        total += b < n ? v : 0;
+        before += b < me ? v : 0;
+      };
+#pragma unroll
+      for (int q = 0; q < kScanBlocks / 4; ++q) {
+        add(q * 4, c[q].x); add(q * 4 + 1, c[q].y); add(q * 4 + 2, c[q].z); add(q * 4 + 3, c[q].w);
       }
     }
   }
@@ -251,7 +331,9 @@ struct Grad {
   int64_t nruns;
   float scale;
   int accumulate;
-  float* part;            // [nruns][2][dim]: a run's piece of a row that began before it, and of one that goes on
+  float* part;            // [nruns][2][part_ld]: a run's piece of a row that began before it, and of one that goes on
+  int part_ld;
+  int64_t cleared;        // rows below this are zeros already
 };
 
 // first position in the sorted list whose row is >= v
@@ -264,29 +346,32 @@ __device__ __forceinline__ int64_t lower_row(const Grad& G, uint32_t v) {
   return lo;
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void put_row(const Grad& G, T* g, const float (&acc)[N]) {
-  Pack<T, N> x;
-  if (G.accumulate) {
-    x = *(const Pack<T, N>*)g;
+// a finished piece of a row of the gradient, from its sum
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void put_row(T* g, const float (&acc)[Piece<T>::N], float scale, int accumulate, int count) {
+  Piece<T> x;
+  if (accumulate) {
+    x = load_piece<WHOLE>(g, count);
 #pragma unroll
-    for (int q = 0; q < N; ++q) x.v[q] = (T)__builtin_fmaf(G.scale, acc[q], (float)x.v[q]);
+    for (int q = 0; q < Piece<T>::N; ++q) x.v[q] = (T)__builtin_fmaf(scale, acc[q], (float)x.v[q]);
   } else {
 #pragma unroll
-    for (int q = 0; q < N; ++q) x.v[q] = (T)(G.scale * acc[q]);
+    for (int q = 0; q < Piece<T>::N; ++q) x.v[q] = (T)(scale * acc[q]);
   }
-  *(Pack<T, N>*)g = x;
+  store_piece<WHOLE>(g, x, count);
 }
 
 constexpr int kZeroRows = 64;   // rows that a block looks up and clears
 
-// blocks [0, sum_blocks): a team of lanes per run and column segment (blockIdx.y); the others clear absent rows
-template <typename T, int N>
+// blocks [0, sum_blocks): a team of lanes per run and column segment (blockIdx.y); the others clear absent rows from
+// `cleared` on
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(Grad G, int64_t sum_blocks, const T* __restrict__ dout,
                                                             int64_t ldd, T* __restrict__ dtable, int64_t ldg) {
+  constexpr int N = Piece<T>::N;
   if (blockIdx.x >= sum_blocks) {
     __shared__ bool present[kZeroRows];
-    const int64_t r0 = (blockIdx.x - sum_blocks) * kZeroRows;
+    const int64_t r0 = G.cleared + (blockIdx.x - sum_blocks) * kZeroRows;
     const int nr = G.rows - r0 < kZeroRows ? (int)(G.rows - r0) : kZeroRows;
     if ((int)threadIdx.x < nr) {
       const uint32_t v = (uint32_t)(r0 + threadIdx.x);
@@ -295,11 +380,10 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(Grad G, int64_t sum_
     }
     __syncthreads();
     const int c0 = (int)blockIdx.y * N << G.lanes_log2, c1 = min(G.dim, c0 + (N << G.lanes_log2));
-    const int per = (c1 - c0) / N;
-    const Pack<T, N> zero{};
+    const int per = (c1 - c0 + N - 1) / N;
     for (int e = threadIdx.x; e < nr * per; e += 256) {
-      const int r = e / per;
-      if (!present[r]) *(Pack<T, N>*)(dtable + (r0 + r) * ldg + c0 + (e - r * per) * N) = zero;
+      const int r = e / per, c = c0 + (e - r * per) * N;
+      if (!present[r]) store_piece<WHOLE>(dtable + (r0 + r) * ldg + c, Piece<T>{}, c1 - c);
     }
     return;
   }
@@ -307,6 +391,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(Grad G, int64_t sum_
   const int64_t run = (int64_t)blockIdx.x * (256 >> G.lanes_log2) + team;
   const int c = ((int)blockIdx.y << G.lanes_log2 | lane) * N;
   if (run >= G.nruns || c >= G.dim) return;
+  const int left = G.dim - c;
   const int64_t i0 = run * G.run, i1 = i0 + G.run < G.n ? i0 + G.run : G.n;
   float acc[N];
 #pragma unroll
@@ -316,9 +401,9 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(Grad G, int64_t sum_
   const auto flush = [&](bool ended) {
     if (cur >= G.rows) return;
     if (began && ended) {
-      put_row<T, N>(G, dtable + (int64_t)cur * ldg + c, acc);
+      put_row<T, WHOLE>(dtable + (int64_t)cur * ldg + c, acc, G.scale, G.accumulate, left);
     } else {
-      float* p = G.part + (run * 2 + (began ? 1 : 0)) * G.dim + c;
+      float* p = G.part + (run * 2 + (began ? 1 : 0)) * G.part_ld + c;   // rows padded to whole pieces
 #pragma unroll
       for (int q = 0; q < N; ++q) p[q] = acc[q];
     }
@@ -326,12 +411,12 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(Grad G, int64_t sum_
   constexpr int U = 8;
   for (int64_t i = i0; i < i1; i += U) {
     uint2 s[U];
-    Pack<T, N> x[U];
+    Piece<T> x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) s[u] = G.sorted[i + u < i1 ? i + u : i1 - 1];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (s[u].x < G.rows) x[u] = *(const Pack<T, N>*)(dout + (int64_t)s[u].y * ldd + c);
+      if (s[u].x < G.rows) x[u] = load_piece<WHOLE>(dout + (int64_t)s[u].y * ldd + c, left);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i + u >= i1) break;
@@ -350,7 +435,8 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(Grad G, int64_t sum_
   flush(i1 == G.n || G.sorted[i1].x != cur);
 }
 
-// A row that crosses runs: the run where it begins adds up its pieces.  4 waves take a quarter of them each, in order.
+// A row that crosses runs: the run where it begins adds up its pieces.  4 waves take a quarter of them each, in order;
+// a lane has 4 columns.
 template <typename T>
 __global__ __launch_bounds__(256) void embedding_join_kernel(Grad G, T* __restrict__ dtable, int64_t ldg) {
   const int64_t run = blockIdx.x;
@@ -359,36 +445,186 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(Grad G, T* __restri
   const uint32_t v = G.sorted[i1 - 1].x;
   if (v >= G.rows || G.sorted[i1].x != v) return;
   if (i0 > 0 && G.sorted[i0].x == v && G.sorted[i0 - 1].x == v) return;   // began in an earlier run
-  const int64_t last = (lower_row(G, v + 1) - 1) / G.run;
-  __shared__ float red[4][64];
+  __shared__ float4 red[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = (int)blockIdx.y * 64 + lane;
-  // pieces: slot 1 of `run`, slot 0 of run + 1 .. last
-  const int64_t count = last - run, per = (count + 3) / 4;
-  float acc = 0.f;
+  // runs that begin with v: 64 looked at together
+  int64_t count = 0;
+  for (;;) {
+    const int64_t at = (run + 1 + count + lane) * G.run;
+    const uint64_t same = __ballot(at < G.n && G.sorted[at < G.n ? at : 0].x == v);
+    count += same == ~0ull ? 64 : __builtin_ctzll(~same);
+    if (same != ~0ull) break;
+  }
+  const int c = ((int)blockIdx.y * 64 + lane) * 4;
+  // pieces: slot 1 of `run`, slot 0 of run + 1 .. run + count
+  const int64_t per = (count + 3) / 4;
+  float4 acc{0.f, 0.f, 0.f, 0.f};
+  const auto add = [&](int64_t slot) {
+    const float4 x = *(const float4*)(G.part + slot * G.part_ld + c);
+    acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+  };
   if (c < G.dim) {
-    if (wave == 0) acc = G.part[(run * 2 + 1) * G.dim + c];
-    const int64_t a = run + 1 + wave * per, b = a + per < last + 1 ? a + per : last + 1;
+    if (wave == 0) add(run * 2 + 1);
+    const int64_t a = run + 1 + wave * per, b = a + per < run + 1 + count ? a + per : run + 1 + count;
 #pragma unroll 8
-    for (int64_t k = a; k < b; ++k) acc += G.part[k * 2 * G.dim + c];
+    for (int64_t k = a; k < b; ++k) add(k * 2);
   }
   red[wave][lane] = acc;
   __syncthreads();
   if (wave == 0 && c < G.dim) {
-    const float one[1] = {((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane]};
-    put_row<T, 1>(G, dtable + (int64_t)v * ldg + c, one);
+    const float4 x = red[0][lane], y = red[1][lane], z = red[2][lane], w = red[3][lane];
+    const float sum[4] = {((x.x + y.x) + z.x) + w.x, ((x.y + y.y) + z.y) + w.y, ((x.z + y.z) + z.z) + w.z,
+                          ((x.w + y.w) + z.w) + w.w};
+    T* g = dtable + (int64_t)v * ldg + c;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (c + q < G.dim) g[q] = (T)(G.accumulate ? __builtin_fmaf(G.scale, sum[q], (float)g[q]) : G.scale * sum[q]);
+  }
+}
+
+// ---- a table of few rows ------------------------------------------------------------------------------------------
+// Blocks sort and sum 256 positions each and leave a sum per row that occurs among them; a second launch adds those
+// up, block after block.  (Per-view codes: 10240 positions, 45 rows, 32 values.)
+constexpr int kFewRows = 64, kFewTile = 256, kFewBits = 7;   // keys 0 .. 64
+
+struct Few {
+  int64_t n;
+  int rows, dim, lanes_log2, accumulate;
+  float scale;
+  int64_t blocks;
+  uint32_t* present;      // [blocks][kFewRows / 32]
+  float* part;            // [blocks][rows][part_ld]
+  int part_ld;
+};
+
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(256) void few_sum_kernel(Ids I, Few F, const T* __restrict__ dout, int64_t ldd) {
+  constexpr int N = Piece<T>::N;
+  __shared__ uint16_t cnt[4][256];
+  __shared__ uint32_t base[256];
+  __shared__ uint32_t wsum[4];
+  __shared__ uint16_t key[kFewTile], pos[kFewTile];
+  __shared__ float cross[256 * N * 2];      // what a team's run has of a row that began before it, and of one that goes on
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = threadIdx.x;
+  const int64_t i0 = (int64_t)blockIdx.x * kFewTile;
+  // sort: rank among the wave's 64 positions by ballots, then the waves in order
+  const uint32_t k = i0 + t < F.n ? key_at(I, i0 + t) : F.rows;    // `rows`: no gradient, sorted last
+  cnt[0][t] = cnt[1][t] = cnt[2][t] = cnt[3][t] = 0;
+  __syncthreads();
+  uint64_t same = ~0ull;
+  for (int b = 0; b < kFewBits; ++b) {
+    const uint64_t m = __ballot((k >> b) & 1);
+    same &= (k >> b) & 1 ? m : ~m;
+  }
+  const uint32_t before = __popcll(same & ((1ull << lane) - 1));
+  if (before == 0) cnt[wave][k] = (uint16_t)__popcll(same);
+  __syncthreads();
+  const uint32_t c0 = cnt[0][t], c1 = cnt[1][t], c2 = cnt[2][t], total = c0 + c1 + c2 + cnt[3][t];
+  uint32_t x = total;
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 63) wsum[wave] = x;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) x += wsum[w];
+  base[t] = x - total;
+  cnt[0][t] = 0; cnt[1][t] = (uint16_t)c0; cnt[2][t] = (uint16_t)(c0 + c1); cnt[3][t] = (uint16_t)(c0 + c1 + c2);
+  const uint64_t there = __ballot(total != 0);
+  if (t < kFewRows && (t & 31) == 0 && blockIdx.y == 0)
+    F.present[blockIdx.x * (kFewRows / 32) + t / 32] =
+        (uint32_t)(there >> (t & 32)) & (F.rows - t >= 32 ? ~0u : F.rows > t ? (1u << (F.rows - t)) - 1 : 0u);
+  __syncthreads();
+  const uint32_t at = base[k] + cnt[wave][k] + before;
+  key[at] = (uint16_t)k;
+  pos[at] = (uint16_t)t;
+  __syncthreads();
+  const int live = (int)base[F.rows];     // positions with a gradient
+  // sums: a team of lanes per run of the sorted positions
+  const int l = t & ((1 << F.lanes_log2) - 1), team = t >> F.lanes_log2, teams = 256 >> F.lanes_log2;
+  const int c = ((int)blockIdx.y << F.lanes_log2 | l) * N, left = F.dim - c;
+  const int run = kFewTile / teams, r0 = team * run, r1 = min(r0 + run, live);
+  float* part = F.part + (int64_t)blockIdx.x * F.rows * F.part_ld + c;
+  float acc[N];
+#pragma unroll
+  for (int q = 0; q < N; ++q) acc[q] = 0.f;
+  const auto keep = [&](float* p) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) p[q] = acc[q];
+  };
+  if (r0 < r1 && left > 0) {
+    int cur = key[r0];
+    bool began = r0 == 0 || key[r0 - 1] != cur;
+    constexpr int U = 8;
+    for (int i = r0; i < r1; i += U) {
+      Piece<T> p[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) p[u] = load_piece<WHOLE>(dout + (i0 + pos[min(i + u, r1 - 1)]) * ldd + c, left);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i + u >= r1) break;
+        if (key[i + u] != cur) {
+          if (began) keep(part + (int64_t)cur * F.part_ld);
+          else keep(cross + t * N);
+          cur = key[i + u];
+          began = true;
+#pragma unroll
+          for (int q = 0; q < N; ++q) acc[q] = 0.f;
+        }
+#pragma unroll
+        for (int q = 0; q < N; ++q) acc[q] += (float)p[u].v[q];
+      }
+    }
+    const bool ended = r1 == live || key[r1] != cur;
+    if (began && ended) keep(part + (int64_t)cur * F.part_ld);
+    else keep(cross + (began ? 256 * N : 0) + t * N);
+  }
+  __syncthreads();
+  // a row that crosses runs: the team where it begins adds the others' pieces, in order
+  if (r0 < r1 && left > 0 && r1 < live) {
+    const int cur = key[r1 - 1];
+    const bool began = r0 == 0 || key[r0] != cur || key[r0 - 1] != cur;
+    if (began && key[r1] == cur) {
+#pragma unroll
+      for (int q = 0; q < N; ++q) acc[q] = cross[256 * N + t * N + q];
+      for (int o = team + 1; o < teams && o * run < live && key[o * run] == cur; ++o)
+#pragma unroll
+        for (int q = 0; q < N; ++q) acc[q] += cross[((o << F.lanes_log2) + l) * N + q];
+      keep(part + (int64_t)cur * F.part_ld);
+    }
+  }
+}
+
+// blockIdx.x: a row; 64 lanes x 4 waves: a lane has a column, a wave a quarter of the blocks
+template <typename T>
+__global__ __launch_bounds__(256) void few_join_kernel(Few F, T* __restrict__ dtable, int64_t ldg) {
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.x;
+  const int c = (int)blockIdx.y * 64 + lane;
+  const int64_t per = (F.blocks + 3) / 4, a = wave * per, b = a + per < F.blocks ? a + per : F.blocks;
+  float acc = 0.f;
+  bool any = false;
+#pragma unroll 8
+  for (int64_t k = a; k < b; ++k) {
+    const bool there = F.present[k * (kFewRows / 32) + r / 32] >> (r & 31) & 1;
+    // a row that does not occur in a block was not written there
+    const float x = F.part[(k * F.rows + r) * F.part_ld + (c < F.dim ? c : 0)];
+    acc += there ? x : 0.f;
+    any |= there;
+  }
+  red[wave][lane] = acc;
+  any = __syncthreads_or(any);
+  if (wave == 0 && c < F.dim && (any || !F.accumulate)) {
+    T* g = dtable + (int64_t)r * ldg + c;
+    const float sum = ((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane];
+    *g = (T)(F.accumulate ? __builtin_fmaf(F.scale, sum, (float)*g) : F.scale * sum);
   }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
-int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
+int piece_of(int dtype) { return dtype == 0 ? 4 : 8; }
 
-bool aligned_rows(const void* p, int64_t ld, int dim, int dtype) {
-  const int e = elem_size(dtype);
-  return ((uintptr_t)p & 15) == 0 && ld * e % 16 == 0 && dim * (int64_t)e % 16 == 0;
-}
-
-// threads per row: enough 16-byte (or single-element) pieces for the row, at most a block
+// threads per row: enough pieces of `n` values for the row, at most a block
 int lanes_for(int dim, int n) {
   int l = 0;
   while (l < 8 && ((int64_t)n << l) < dim) ++l;
@@ -404,63 +640,78 @@ int check_ids(const char* fn, const void* ids, int64_t stride, int64_t n, int64_
 }
 
 struct Plan {
-  int bits, passes, run, lanes_log2, vec;
-  int64_t nblk, nruns, pairs, counts, part, total;   // byte offsets: pairs of the second buffer, ...
+  bool few;
+  int bits, passes, run, lanes_log2, part_ld;
+  int64_t nblk, nruns, pairs, counts, part, total;   // byte offsets: the pairs' second buffer, ...
 };
 
-Plan plan_for(int64_t n, int64_t rows, int dim, int dtype, bool wide) {
+Plan plan_for(int64_t n, int64_t rows, int dim, int dtype) {
   Plan p{};
+  const auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
+  const int N = piece_of(dtype);
+  p.lanes_log2 = lanes_for(dim, N);
+  p.part_ld = (dim + N - 1) / N * N;
+  // Few rows: two launches instead of four to six, as long as the blocks' sums (rows of 256 positions) are less than the
+  // positions themselves and a row's wave has no more than 64 blocks to add up.
+  p.few = n > 0 && rows <= kFewRows && n <= 256 * kFewTile && dim <= 4096;
+  if (p.few) {
+    p.lanes_log2 = p.lanes_log2 < 5 ? p.lanes_log2 : 5;   // 8 teams or more to a block: runs of 32 positions or fewer
+    p.nblk = (n + kFewTile - 1) / kFewTile;
+    p.part = up(p.nblk * (kFewRows / 32) * 4);
+    p.total = p.part + up(p.nblk * rows * p.part_ld * 4);
+    return p;
+  }
   int need = 1;
   while ((rows >> need) != 0) ++need;      // keys 0 .. rows
   p.passes = (need + kMaxBits - 1) / kMaxBits;
   p.bits = (need + p.passes - 1) / p.passes;
-  p.vec = wide ? 16 / elem_size(dtype) : 1;
-  p.lanes_log2 = lanes_for(dim, p.vec);
   p.nblk = (n + kTileRounds * kSortThreads - 1) / (kTileRounds * kSortThreads);
-  p.run = 64;
-  while (p.run > 8 && (n / p.run) << p.lanes_log2 < 256 * 1024) p.run >>= 1;
+  // 512 blocks of teams if there are positions enough (9001 x 771: 56 us with runs of 16, 63, 78, 111 with 32, 64, 128)
+  p.run = 128;
+  while (p.run > 8 && (n / p.run) << p.lanes_log2 < 128 * 1024) p.run >>= 1;
   p.nruns = (n + p.run - 1) / p.run;
-  const auto up = [](int64_t b) { return (b + 255) / 256 * 256; };
   p.pairs = up(n * 8);
   p.counts = p.pairs * 2;
-  p.part = p.counts + up((p.nblk + 1) * 4 << p.bits);
-  p.total = p.part + up(p.nruns * 2 * dim * 4);
+  p.part = p.counts + up((p.nblk + 3) / 4 * 4 * 4 << p.bits) + (4 << p.bits);   // the digits' totals last
+  p.total = p.part + up(p.nruns * 2 * p.part_ld * 4);
   return p;
 }
 
 template <typename T>
-int launch_fwd(const Ids& I, int64_t n, const void* table, int64_t ldt, int dim, float scale, void* out, int64_t ldo,
-               bool wide, hipStream_t s) {
-  constexpr int V = Vec16<T>::N;
-  const int vec = wide ? V : 1, l = lanes_for(dim, vec), per = 256 >> l;
-  const dim3 grid((unsigned)((n + per - 1) / per), (unsigned)((dim + (vec << l) - 1) / (vec << l)));
-  if (wide)
-    hipLaunchKernelGGL((embedding_fwd_kernel<T, V>), grid, dim3(256), 0, s, I, n, (const T*)table, ldt, dim, l, scale,
-                       (T*)out, ldo);
-  else
-    hipLaunchKernelGGL((embedding_fwd_kernel<T, 1>), grid, dim3(256), 0, s, I, n, (const T*)table, ldt, dim, l, scale,
-                       (T*)out, ldo);
-  return 0;
+void launch_fwd(const Ids& I, int64_t n, const void* table, int64_t ldt, int dim, float scale, void* out, int64_t ldo,
+                hipStream_t s) {
+  constexpr int N = Piece<T>::N;
+  // 4 rows a team once there are blocks enough
+  const int l = lanes_for(dim, N), segs = (dim + (N << l) - 1) / (N << l);
+  const bool many = (n << l) * segs >= 4 * 256 * 2048;
+  const int per = (256 >> l) * (many ? 4 : 1);
+  const dim3 grid((unsigned)((n + per - 1) / per), (unsigned)segs);
+  const auto kernel = dim % N == 0 ? many ? embedding_fwd_kernel<T, true, 4> : embedding_fwd_kernel<T, true, 1>
+                                   : many ? embedding_fwd_kernel<T, false, 4> : embedding_fwd_kernel<T, false, 1>;
+  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, I, n, (const T*)table, ldt, dim, l, scale, (T*)out, ldo);
 }
 
 template <typename T>
-int launch_sums(const Grad& G, const Plan& p, const T* dout, int64_t ldd, T* dtable, int64_t ldg, hipStream_t s) {
-  constexpr int V = Vec16<T>::N;
-  const int per = 256 >> p.lanes_log2;
+void launch_few(const Ids& I, const Few& F, const void* dout, int64_t ldd, void* dtable, int64_t ldg, hipStream_t s) {
+  const int seg = Piece<T>::N << F.lanes_log2;
+  const auto kernel = F.dim % Piece<T>::N == 0 ? few_sum_kernel<T, true> : few_sum_kernel<T, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)F.blocks, (unsigned)((F.dim + seg - 1) / seg)), dim3(256), 0, s,
+                     I, F, (const T*)dout, ldd);
+  hipLaunchKernelGGL((few_join_kernel<T>), dim3((unsigned)F.rows, (unsigned)((F.dim + 63) / 64)), dim3(256), 0, s, F,
+                     (T*)dtable, ldg);
+}
+
+template <typename T>
+void launch_sums(const Grad& G, const void* dout, int64_t ldd, void* dtable, int64_t ldg, hipStream_t s) {
+  const int per = 256 >> G.lanes_log2, seg = Piece<T>::N << G.lanes_log2;
   const int64_t sums = (G.nruns + per - 1) / per;
-  const int64_t zeros = G.accumulate ? 0 : (G.rows + kZeroRows - 1) / kZeroRows;
-  const unsigned segs = (unsigned)((G.dim + (p.vec << p.lanes_log2) - 1) / (p.vec << p.lanes_log2));
-  if (sums + zeros == 0) return 0;
-  if (p.vec > 1)
-    hipLaunchKernelGGL((embedding_sum_kernel<T, V>), dim3((unsigned)(sums + zeros), segs), dim3(256), 0, s, G, sums,
-                       dout, ldd, dtable, ldg);
-  else
-    hipLaunchKernelGGL((embedding_sum_kernel<T, 1>), dim3((unsigned)(sums + zeros), segs), dim3(256), 0, s, G, sums,
-                       dout, ldd, dtable, ldg);
+  const int64_t zeros = G.accumulate ? 0 : (G.rows - G.cleared + kZeroRows - 1) / kZeroRows;
+  const auto kernel = G.dim % Piece<T>::N == 0 ? embedding_sum_kernel<T, true> : embedding_sum_kernel<T, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(sums + zeros), (unsigned)((G.dim + seg - 1) / seg)),
+                     dim3(256), 0, s, G, sums, (const T*)dout, ldd, (T*)dtable, ldg);
   if (G.nruns > 1)
-    hipLaunchKernelGGL((embedding_join_kernel<T>), dim3((unsigned)(G.nruns - 1), (unsigned)((G.dim + 63) / 64)),
-                       dim3(256), 0, s, G, dtable, ldg);
-  return 0;
+    hipLaunchKernelGGL((embedding_join_kernel<T>), dim3((unsigned)(G.nruns - 1), (unsigned)((G.dim + 255) / 256)),
+                       dim3(256), 0, s, G, (T*)dtable, ldg);
 }
 
 }  // namespace
@@ -474,11 +725,10 @@ MMS_EXPORT int mms_embedding_fwd(const void* ids, int ids64, int64_t ids_stride,
   if (n == 0) return 0;
   MMS_REQUIRE(table && out && ldt >= dim && ldo >= dim, fn, "null table or output, or rows that do not fit");
   const Ids I{ids, ids_stride, ids64, rows, -1};
-  const bool wide = aligned_rows(table, ldt, dim, dtype) && aligned_rows(out, ldo, dim, dtype);
   hipStream_t s = mms::as_stream(stream);
-  if (dtype == 0) launch_fwd<float>(I, n, table, ldt, dim, scale, out, ldo, wide, s);
-  else if (dtype == 1) launch_fwd<bf16_t>(I, n, table, ldt, dim, scale, out, ldo, wide, s);
-  else launch_fwd<_Float16>(I, n, table, ldt, dim, scale, out, ldo, wide, s);
+  if (dtype == 0) launch_fwd<float>(I, n, table, ldt, dim, scale, out, ldo, s);
+  else if (dtype == 1) launch_fwd<bf16_t>(I, n, table, ldt, dim, scale, out, ldo, s);
+  else launch_fwd<_Float16>(I, n, table, ldt, dim, scale, out, ldo, s);
   return mms::check_launch(fn);
 }
 
@@ -487,8 +737,7 @@ MMS_EXPORT int mms_embedding_bwd_workspace(int64_t n, int64_t rows, int dim, int
   const int rc = check_ids(fn, fn, 0, n, rows, dim, dtype);
   if (rc) return rc;
   MMS_REQUIRE(bytes != nullptr, fn, "null output");
-  const int64_t a = plan_for(n, rows, dim, dtype, true).total, b = plan_for(n, rows, dim, dtype, false).total;
-  *bytes = a > b ? a : b;
+  *bytes = plan_for(n, rows, dim, dtype).total;
   return 0;
 }
 
@@ -501,37 +750,68 @@ MMS_EXPORT int mms_embedding_bwd(const void* ids, int ids64, int64_t ids_stride,
   MMS_REQUIRE(dtable && ldg >= dim && (n == 0 || (dout && ldd >= dim)), fn,
               "null gradients, or rows that do not fit");
   if (n == 0 && accumulate) return 0;
-  const bool wide = aligned_rows(dtable, ldg, dim, dtype) && (n == 0 || aligned_rows(dout, ldd, dim, dtype));
-  const Plan p = plan_for(n, rows, dim, dtype, wide);
+  const Plan p = plan_for(n, rows, dim, dtype);
   MMS_REQUIRE(p.total == 0 || n == 0 || (ws && ws_bytes >= p.total && ((uintptr_t)ws & 255) == 0), fn,
               "workspace too small (mms_embedding_bwd_workspace) or not 256-byte aligned");
   hipStream_t s = mms::as_stream(stream);
   const Ids I{ids, ids_stride, ids64, rows, padding_idx};
   char* w = (char*)ws;
+  if (p.few) {
+    const Few F{n, (int)rows, dim, p.lanes_log2, accumulate, scale, p.nblk, (uint32_t*)w, (float*)(w + p.part), p.part_ld};
+    if (dtype == 0) launch_few<float>(I, F, dout, ldd, dtable, ldg, s);
+    else if (dtype == 1) launch_few<bf16_t>(I, F, dout, ldd, dtable, ldg, s);
+    else launch_few<_Float16>(I, F, dout, ldd, dtable, ldg, s);
+    return mms::check_launch(fn);
+  }
   uint2* buf[2] = {(uint2*)w, (uint2*)(w + p.pairs)};
   uint32_t* counts = (uint32_t*)(w + p.counts);
-  uint32_t* totals = counts + (p.nblk << p.bits);
+  const int ld = (int)((p.nblk + 3) / 4 * 4);
+  uint32_t* totals = counts + ((int64_t)ld << p.bits);
   const uint2* sorted = buf[0];
-  if (n > 0 && n <= kOneRounds * kSortThreads) {
-    hipLaunchKernelGGL(sort_one_kernel, dim3(1), dim3(kSortThreads), 0, s, I, (int)n, p.bits, p.passes, buf[0]);
+  const bool one = n <= kOneRounds * kSortThreads;
+  // As much as hides in the sort's launches, in one of a single block or two for each digit (9001 indices below 50257, 771
+  // wide: 70 us with nothing cleared there, 63 with 24 MB a launch, 56 with 48; 65536 below 131072, 2048 wide: 197, 192,
+  // 189, and 196 with 136 MB, all of the table).
+  const int es = dtype == 0 ? 4 : 2, launches = one ? 1 : 2 * p.passes;
+  const int64_t row_bytes = (int64_t)dim * es;
+  const int64_t share = one ? ((n + kSortThreads - 1) / kSortThreads * p.passes * 5 + 10) << 20 : 48 << 20;
+  int64_t cleared = accumulate || n == 0 ? 0 : launches * share / row_bytes;
+  if (cleared > rows) cleared = rows;
+  const int64_t each = (cleared + launches - 1) / launches;
+  int64_t begun = 0;
+  // the next launch's share of the rows, and its blocks behind `first` others
+  const auto zeros = [&](int64_t first, unsigned& blocks) {
+    Zeros Z{(char*)dtable + begun * ldg * es, begun + each < cleared ? each : cleared - begun, row_bytes, ldg * es, (int)first};
+    begun += Z.rows;
+    const int64_t pieces = Z.ld == Z.bytes ? (Z.rows * Z.bytes + 15) / 16 : Z.rows * ((Z.bytes + 15) / 16);
+    blocks = (unsigned)(first + (pieces + kZeroChunk / 16 - 1) / (kZeroChunk / 16));
+    return Z;
+  };
+  unsigned blocks = 0;
+  if (n > 0 && one) {
+    const Zeros Z = zeros(1, blocks);
+    hipLaunchKernelGGL(sort_one_kernel, dim3(blocks), dim3(kSortThreads), 0, s, I, (int)n, p.bits, p.passes, buf[0], Z);
   } else if (n > 0) {
     const uint2* in = nullptr;
     for (int k = 0; k < p.passes; ++k) {
       const bool scan = p.nblk > kScanBlocks;
-      hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)p.nblk), dim3(kSortThreads), 0, s, I, in, n, p.bits,
-                         k * p.bits, counts);
+      Zeros Z = zeros(p.nblk, blocks);
+      hipLaunchKernelGGL(sort_count_kernel, dim3(blocks), dim3(kSortThreads), 0, s, I, in, n, p.bits, k * p.bits, counts,
+                         ld, Z);
       if (scan)
-        hipLaunchKernelGGL(sort_scan_kernel, dim3(1u << p.bits), dim3(kSortThreads), 0, s, counts, (int)p.nblk, p.bits,
+        hipLaunchKernelGGL(sort_scan_kernel, dim3(1u << p.bits), dim3(kSortThreads), 0, s, counts, (int)p.nblk, ld,
                            totals);
-      hipLaunchKernelGGL(sort_scatter_kernel, dim3((unsigned)p.nblk), dim3(kSortThreads), 0, s, I, in, n, p.bits,
-                         k * p.bits, counts, scan ? totals : nullptr, buf[k & 1]);
+      Z = zeros(p.nblk, blocks);
+      hipLaunchKernelGGL(sort_scatter_kernel, dim3(blocks), dim3(kSortThreads), 0, s, I, in, n, p.bits, k * p.bits,
+                         counts, ld, scan ? totals : nullptr, buf[k & 1], (int)p.nblk, Z);
       in = buf[k & 1];
     }
     sorted = in;
   }
-  const Grad G{sorted, n, rows, dim, p.lanes_log2, p.run, p.nruns, scale, accumulate, (float*)(w + p.part)};
-  if (dtype == 0) launch_sums<float>(G, p, (const float*)dout, ldd, (float*)dtable, ldg, s);
-  else if (dtype == 1) launch_sums<bf16_t>(G, p, (const bf16_t*)dout, ldd, (bf16_t*)dtable, ldg, s);
-  else launch_sums<_Float16>(G, p, (const _Float16*)dout, ldd, (_Float16*)dtable, ldg, s);
+  const Grad G{sorted, n, rows, dim, p.lanes_log2, p.run, p.nruns, scale, accumulate, (float*)(w + p.part), p.part_ld,
+               cleared};
+  if (dtype == 0) launch_sums<float>(G, dout, ldd, dtable, ldg, s);
+  else if (dtype == 1) launch_sums<bf16_t>(G, dout, ldd, dtable, ldg, s);
+  else launch_sums<_Float16>(G, dout, ldd, dtable, ldg, s);
   return mms::check_launch(fn);
 }

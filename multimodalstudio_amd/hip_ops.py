@@ -5,7 +5,9 @@ Every function here requires CUDA(HIP) tensors and raises otherwise: there is no
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 import os
 from typing import Optional
 
@@ -227,19 +229,17 @@ NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # torch.optim.Muon's quintic
 _MATRIX_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
-class _on_device:
-    """The device of ``t`` as the current one (a no-op if it is already): streams and launches go to it."""
+_HERE = contextlib.nullcontext()
 
-    def __init__(self, t: torch.Tensor):
-        self.guard = None if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
+def _stream_of(t: torch.Tensor) -> int:
+    """The current stream of ``t``'s device (torch.cuda.current_stream's handle at a fifth of its host time)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+
+def _on_device(t: torch.Tensor):
+    """The device of ``t`` as the current one (nothing to do if it is already): streams and launches go to it."""
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def _matrices(t: torch.Tensor, what: str, copy: bool):
@@ -326,7 +326,7 @@ def newton_schulz(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float
             o = _MatrixTable([_matrices(outs[i], "newton_schulz: result", False) for i in pick])
             ws = _muon_workspace(g, p, mats[0].device)
             _lib.call("mms_newton_schulz", g.n, g.batch, g.rows, g.cols, g.ptr, g.ld, g.bs, o.ptr, o.ld, o.bs, bf16, p,
-                      int(steps), a, b, c, float(eps), ws.data_ptr(), ws.numel(), _stream())
+                      int(steps), a, b, c, float(eps), ws.data_ptr(), ws.numel(), _stream_of(mats[0]))
     return outs
 
 
@@ -391,7 +391,7 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
             _lib.call("mms_muon_step", w.n, w.batch, w.rows, w.cols, w.ptr, w.ld, w.bs, g.ptr, g.ld, g.bs, m, scale,
                       bf16, pr, int(steps), a, b, c, float(eps), float(momentum), int(bool(nesterov)), _ptr(sumsq),
                       float(max_norm), _ptr(hyper), 1.0 - float(lr) * float(weight_decay), -float(lr), ws.data_ptr(),
-                      ws.numel(), _stream())
+                      ws.numel(), _stream_of(params[0]))
 
 
 # ----------------------------------------------------------------------------------------------
@@ -400,46 +400,55 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
 _TABLE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _check_table(ids: torch.Tensor, rows: torch.Tensor, what: str):
-    _check_dev(ids, rows)
-    if ids.dtype not in (torch.int32, torch.int64):
+def _check_table(ids: torch.Tensor, rows: torch.Tensor, what: str) -> int:
+    if not (ids.is_cuda and rows.is_cuda):
+        _check_dev(ids, rows)
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         raise TypeError(f"embedding: indices must be int32 or int64, got {ids.dtype}")
-    if rows.dtype not in _TABLE_DTYPES:
+    dt = _TABLE_DTYPES.get(rows.dtype)
+    if dt is None:
         raise TypeError(f"embedding: {what} must be float32, bfloat16 or float16, got {rows.dtype}")
-    if ids.device != rows.device:
+    if ids.get_device() != rows.get_device():
         raise ValueError(f"embedding: indices on {ids.device}, {what} on {rows.device}")
+    return dt
 
 
 def _flat_ids(ids: torch.Tensor):
     """(tensor, elements between two indices): a column of a coordinate tensor is read where it lies."""
-    n = ids.numel()
     if ids.is_contiguous():
         return ids, 1
     lead = [(s, st) for s, st in zip(ids.shape, ids.stride()) if s != 1]
-    if n and len(lead) == 1 and lead[0][1] > 0:
+    if ids.numel() and len(lead) == 1 and lead[0][1] > 0:
         return ids, lead[0][1]
     return ids.contiguous(), 1
 
 
 def _rows2d(t: torch.Tensor, dim: int) -> torch.Tensor:
-    t = t.reshape(-1, dim)
+    t = t.reshape(-1, dim) if t.dim() != 2 else t
     return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= dim) else t.contiguous()
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """out[..., :] = scale * table[ids[...], :]; ids int32 / int64 of any shape, table [rows, dim] float32, bfloat16 or
     float16.  An index outside the table gives a row of zeros."""
-    _check_table(ids, table, "the table")
+    dt = _check_table(ids, table, "the table")
     if table.dim() != 2 or table.shape[0] == 0 or table.shape[1] == 0:
         raise ValueError(f"embedding: the table must be [rows, dim], got {tuple(table.shape)}")
-    t = table if table.stride(1) == 1 and table.stride(0) >= table.shape[1] else table.contiguous()
-    out = torch.empty(*ids.shape, table.shape[1], dtype=table.dtype, device=table.device)
+    rows, dim = table.shape
+    t = table if table.is_contiguous() or (table.stride(1) == 1 and table.stride(0) >= dim) else table.contiguous()
+    out = torch.empty(*ids.shape, dim, dtype=table.dtype, device=table.device)
     flat, stride = _flat_ids(ids)
     with _on_device(t):
-        _lib.call("mms_embedding_fwd", flat.data_ptr(), int(ids.dtype == torch.int64), stride, ids.numel(),
-                  t.data_ptr(), t.stride(0), t.shape[0], t.shape[1], _TABLE_DTYPES[t.dtype], float(scale),
-                  out.data_ptr(), t.shape[1], _stream())
+        _lib.call("mms_embedding_fwd", flat.data_ptr(), ids.dtype is torch.int64, stride, ids.numel(), t.data_ptr(),
+                  dim if rows == 1 else t.stride(0), rows, dim, dt, scale, out.data_ptr(), dim, _stream_of(t))
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _embedding_workspace(n: int, rows: int, dim: int, dt: int) -> int:
+    need = ctypes.c_int64(0)
+    _lib.call("mms_embedding_bwd_workspace", n, rows, dim, dt, ctypes.addressof(need))
+    return max(1, need.value)
 
 
 def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: float = 1.0,
@@ -449,9 +458,9 @@ def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: 
     fp32 and in an order that ``ids`` alone fixes (the same bits on each call).  Positions whose index is
     ``padding_idx`` or outside the table add nothing, whatever ``dout`` holds there.  ``out``: written in place, or
     added into with ``accumulate``."""
-    _check_table(ids, dout, "the gradient")
+    dt = _check_table(ids, dout, "the gradient")
     dim = dout.shape[-1] if dout.dim() else 0
-    if dim == 0 or tuple(dout.shape[:-1]) != tuple(ids.shape) or rows < 1:
+    if dim == 0 or dout.shape[:-1] != ids.shape or rows < 1:
         raise ValueError(f"embedding_backward: indices {tuple(ids.shape)} need a gradient [..., dim], got "
                          f"{tuple(dout.shape)} for {rows} rows")
     if out is None:
@@ -462,21 +471,20 @@ def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: 
             (dim > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < dim):
         raise ValueError(f"embedding_backward: out must be [{rows}, {dim}] {dout.dtype} with contiguous rows on "
                          f"{dout.device}")
+    pad = -1
     if padding_idx is not None:
         if not -rows <= padding_idx < rows:
             raise ValueError(f"embedding_backward: padding_idx {padding_idx} is outside the table's {rows} rows")
-        padding_idx = padding_idx % rows
+        pad = padding_idx % rows
     d = _rows2d(dout, dim)
     flat, stride = _flat_ids(ids)
-    dt = _TABLE_DTYPES[dout.dtype]
-    need = ctypes.c_int64(0)
-    _lib.call("mms_embedding_bwd_workspace", ids.numel(), int(rows), dim, dt, ctypes.addressof(need))
+    n = ids.numel()
+    need = _embedding_workspace(n, rows, dim, dt)
     with _on_device(dout):
-        ws = torch.empty(max(1, need.value), dtype=torch.uint8, device=dout.device)
-        _lib.call("mms_embedding_bwd", flat.data_ptr(), int(ids.dtype == torch.int64), stride, ids.numel(),
-                  d.data_ptr(), dim if d.shape[0] <= 1 else d.stride(0), int(rows), dim, dt, float(scale),
-                  -1 if padding_idx is None else int(padding_idx), out.data_ptr(), dim if rows == 1 else out.stride(0),
-                  int(bool(accumulate)), ws.data_ptr(), ws.numel(), _stream())
+        ws = torch.empty(need, dtype=torch.uint8, device=dout.device)
+        _lib.call("mms_embedding_bwd", flat.data_ptr(), ids.dtype is torch.int64, stride, n, d.data_ptr(),
+                  dim if n <= 1 else d.stride(0), rows, dim, dt, scale, pad, out.data_ptr(),
+                  dim if rows == 1 else out.stride(0), bool(accumulate), ws.data_ptr(), need, _stream_of(dout))
     return out
 
 

@@ -101,7 +101,9 @@ def test_embedding_refusals(L):
     need = ctypes.c_int64(-1)
     assert L.mms_embedding_bwd_workspace(0, 5, 8, 0, ctypes.addressof(need)) == 0
     assert L.mms_embedding_bwd_workspace(1000, 5, 8, 0, None) != 0
-    assert L.mms_embedding_bwd_workspace(1000, 5, 8, 0, ctypes.addressof(need)) == 0 and need.value > 2 * 8000
+    # many rows: two lists of (row, position); few: a sum per row and 256 positions
+    assert L.mms_embedding_bwd_workspace(1000, 500, 8, 0, ctypes.addressof(need)) == 0 and need.value > 2 * 8000
+    assert L.mms_embedding_bwd_workspace(1000, 5, 8, 0, ctypes.addressof(need)) == 0 and need.value >= 4 * 5 * 8 * 4
 
 
 def test_python_entry_points_refuse_host_tensors():

@@ -19,8 +19,8 @@ def gen(dev):
 
 
 def plain_sums(ids, dout, rows, scale, pad=None):
-    """(gradient, bound on |error|) in 64 bits."""
-    ids, d = ids.reshape(-1).long(), dout.reshape(-1, dout.shape[-1]).double()
+    """(gradient, bound on |error|) in 64 bits, on the host."""
+    ids, d = ids.reshape(-1).long().cpu(), dout.reshape(-1, dout.shape[-1]).cpu().double()
     live = (ids >= 0) & (ids < rows)
     if pad is not None:
         live &= ids != pad
@@ -34,10 +34,10 @@ def plain_sums(ids, dout, rows, scale, pad=None):
 def check(got, ids, dout, rows, scale=1.0, pad=None, base=None):
     want, tol = plain_sums(ids, dout, rows, scale, pad)
     if base is not None:
-        want = want + base.double()
+        want = want + base.cpu().double()
         tol = tol + (2.0 ** -24 + HALF[dout.dtype]) * want.abs()
     assert got.shape == want.shape and got.dtype == dout.dtype
-    bad = ~((got.double() - want).abs() <= tol)
+    bad = ~((got.cpu().double() - want).abs() <= tol)
     assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist())
 
 
@@ -64,6 +64,9 @@ def draw_ids(kind, n, rows, gen):
     (4096, 1023, 24, "uniform"), (5000, 1024, 40, "outside"), (12288, 45, 32, "skewed"), (12289, 45, 32, "skewed"),
     (9001, 50257, 77, "skewed"), (20000, 2000, 771, "uniform"), (40000, 5, 64, "same"), (40000, 300, 96, "reversed"),
     (30000, 131072, 256, "skewed"), (300000, 1000, 8, "skewed"), (270000, 2097153, 2, "outside"),
+    # a table of few rows (64 at most): its last size, one more row, one more position than its blocks take, wide rows
+    (255, 64, 5, "uniform"), (5000, 64, 130, "outside"), (5000, 65, 130, "outside"), (65536, 45, 33, "skewed"),
+    (65537, 45, 33, "skewed"), (4097, 10, 4096, "reversed"), (4097, 10, 4097, "reversed"), (4095, 63, 8, "sorted"),
 ])
 def test_lookup_and_gradient(dev, gen, n, rows, dim, kind, dtype):
     from multimodalstudio_amd import hip_ops
