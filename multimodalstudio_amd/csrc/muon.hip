@@ -113,8 +113,8 @@ __device__ __forceinline__ int find_item(const NsArgs& A, int blk) {
   const bool before = lane < A.n && A.blk0[lane < kNsItems ? lane : 0] <= blk;
   return __builtin_amdgcn_readfirstlane(__popcll(__ballot(before)) - 1);
 }
-__device__ __forceinline__ int find_item(const NsTable* T, int map, int blk, int& first) {
-  const int b0 = T->blk0[map][threadIdx.x & 63];
+__device__ __forceinline__ int find_item(const NsTable* T, int map, int& first) {
+  const int blk = blockIdx.x, b0 = T->blk0[map][threadIdx.x & 63];
   const int i = __builtin_amdgcn_readfirstlane(__popcll(__ballot(b0 <= blk)) - 1);
   first = __builtin_amdgcn_readlane(b0, i);
   return i;
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const NsTable* __restrict_
   __shared__ float t[64][65];
   __shared__ double red[4];
   int first;
-  const NsItem it = load_item(T, find_item(T, MAP_PACK, blockIdx.x, first));
+  const NsItem it = load_item(T, find_item(T, MAP_PACK, first));
   const NsLayout L(it.rows, it.cols, W);
   const bool tall = it.rows > it.cols;
   const int tr = (tall ? L.cp : L.rp) / 64, tc = (tall ? L.rp : L.cp) / 64;
@@ -265,6 +265,47 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const NsTable* __restrict_
   const int k = q / (tr * tc), i0 = (q / tc) % tr * 64, j0 = q % tc * 64;
   gchar* ws = (gchar*)it.ws + k * L.bytes();
   const int64_t n = (int64_t)it.rows * it.cols;
+  const gchar* g = (const gchar*)it.g + k * it.bsg * (bf16 ? 2 : 4);
+  const MMS_GLOBAL float* m = it.m ? (const MMS_GLOBAL float*)it.m + k * n : nullptr;
+  const float clip = clip_of(S), mu = S.momentum;
+  // u, 16 values a thread: 4 columns of 4 rows, or 1 of 16 where rows are not whole 16 bytes (8 of bf16)
+  float gv[16], mv[16];
+  const bool quads = it.cols % 4 == 0 && it.ldg % 4 == 0 && ((uint64_t)g & (bf16 ? 7 : 15)) == 0 && ((uint64_t)m & 15) == 0;
+  const int lane16 = threadIdx.x & 15, lane64 = threadIdx.x & 63;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) gv[e] = mv[e] = 0.f;
+  if (quads) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = i0 + e * 16 + (threadIdx.x >> 4), j = j0 + lane16 * 4;
+      if (i < it.rows && j < it.cols) {
+        const int64_t at = (int64_t)i * it.ldg + j;
+        if (bf16) {
+          const uint64_t v = *(const MMS_GLOBAL uint64_t*)(g + at * 2);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) gv[e * 4 + z] = __uint_as_float((uint32_t)(v >> (16 * z)) << 16);
+        } else {
+          const floatx4 v = *(const MMS_GLOBAL floatx4*)(g + at * 4);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) gv[e * 4 + z] = v[z];
+        }
+        if (m) {
+          const floatx4 v = *(const MMS_GLOBAL floatx4*)(m + (int64_t)i * it.cols + j);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) mv[e * 4 + z] = v[z];
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int i = i0 + e * 4 + (threadIdx.x >> 6), j = j0 + lane64;
+      if (i < it.rows && j < it.cols) {
+        gv[e] = load1(g, (int64_t)i * it.ldg + j, bf16);
+        if (m) mv[e] = m[(int64_t)i * it.cols + j];
+      }
+    }
+  }
   // |u|: the partial sums in a fixed order
   const int nb = norm_blocks(it.rows, it.cols);
   double sum = 0.0;
@@ -275,23 +316,12 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const NsTable* __restrict_
   double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
   norm = norm < S.eps ? S.eps : norm;
   const double inv = (double)kScale / norm;
-
-  const gchar* g = (const gchar*)it.g + k * it.bsg * (bf16 ? 2 : 4);
-  const MMS_GLOBAL float* m = it.m ? (const MMS_GLOBAL float*)it.m + k * n : nullptr;
-  const float clip = clip_of(S), mu = S.momentum;
-  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-    const int i = i0 + (e >> 6), j = j0 + (e & 63);
-    float u = 0.f;
-    if (i < it.rows && j < it.cols) {
-      const float gi = load1(g, (int64_t)i * it.ldg + j, bf16) * clip;
-      u = gi;
-      if (m) {
-        const float mi = m[(int64_t)i * it.cols + j];
-        u = S.nesterov ? __builtin_fmaf(mu, mi - gi, gi) : mi;
-      }
-      u = (float)(u * inv);
-    }
-    t[e >> 6][e & 63] = u;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const float gi = gv[e] * clip;
+    const float u = !m ? gi : S.nesterov ? __builtin_fmaf(mu, mv[e] - gi, gi) : mv[e];
+    const int i = quads ? (e >> 2) * 16 + (threadIdx.x >> 4) : e * 4 + (threadIdx.x >> 6);
+    t[i][quads ? lane16 * 4 + (e & 3) : lane64] = (float)(u * inv);
   }
   __syncthreads();
   // the tile in its own order is X (wide) or X^T (tall); the other one gets the transposed tile
@@ -349,7 +379,7 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
   __shared__ __attribute__((aligned(1024))) char lds[NBUF * STAGE > SLAB ? NBUF * STAGE : SLAB];
 
   int first;
-  const NsItem it = load_item(T, find_item(T, PHASE == PHASE_A ? MAP_A : PHASE == PHASE_B ? MAP_B : MAP_X, blockIdx.x, first));
+  const NsItem it = load_item(T, find_item(T, PHASE == PHASE_A ? MAP_A : PHASE == PHASE_B ? MAP_B : MAP_X, first));
   const NsLayout L(it.rows, it.cols, W);
   const int nr = (L.rp + TILE - 1) / TILE, nc = (L.cp + TILE - 1) / TILE;
   const int per = PHASE <= PHASE_B ? nr * (nr + 1) / 2 : nr * nc;
@@ -491,11 +521,41 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
   gchar* out = PHASE == PHASE_LAST ? (gchar*)it.p + k * it.bsp * (bf16 ? 2 : 4) : nullptr;
   const float decay = PHASE == PHASE_LAST && it.m ? (S.hyper ? S.hyper[0] : S.decay) : 0.f;
   const float gain = PHASE == PHASE_LAST ? (it.m ? (S.hyper ? S.hyper[1] : S.neg_lr) * it.scale : 1.f) * kDescale : 0.f;
-  const auto put = [&](int row, int col, float v) {   // row, col of the caller's matrix
+  // 4 values to the caller's matrix, together where its rows are whole and aligned groups of 4
+  const bool quads = PHASE == PHASE_LAST && it.cols % 4 == 0 && it.ldp % 4 == 0 && ((uint64_t)out & (bf16 ? 7 : 15)) == 0;
+  const auto put = [&](int row, int col, const float* v) {
+    if (row >= it.rows || col >= it.cols) return;
     const int64_t e = (int64_t)row * it.ldp + col;
-    v *= gain;
-    if (it.m) v = __builtin_fmaf(load1(out, e, bf16), decay, v);
-    store1(out, e, bf16, v);
+    float y[4];
+    if (quads) {
+      MMS_GLOBAL uint64_t* p16 = (MMS_GLOBAL uint64_t*)(out + e * 2);
+      MMS_GLOBAL floatx4* p32 = (MMS_GLOBAL floatx4*)(out + e * 4);
+      floatx4 old{0.f, 0.f, 0.f, 0.f};
+      if (it.m) {
+        if (bf16) {
+          const uint64_t w = *p16;
+#pragma unroll
+          for (int z = 0; z < 4; ++z) old[z] = __uint_as_float((uint32_t)(w >> (16 * z)) << 16);
+        } else {
+          old = *p32;
+        }
+      }
+#pragma unroll
+      for (int z = 0; z < 4; ++z) y[z] = it.m ? __builtin_fmaf(old[z], decay, v[z] * gain) : v[z] * gain;
+      if (bf16) {
+        uint64_t w = 0;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) w |= (uint64_t)to_bf16(y[z]) << (16 * z);
+        *p16 = w;
+      } else {
+        *p32 = floatx4{y[0], y[1], y[2], y[3]};
+      }
+      return;
+    }
+#pragma unroll
+    for (int z = 0; z < 4; ++z)
+      if (col + z < it.cols)
+        store1(out, e + z, bf16, it.m ? __builtin_fmaf(load1(out, e + z, bf16), decay, v[z] * gain) : v[z] * gain);
   };
   const int width = PHASE <= PHASE_B ? L.rp : L.cp;
   for (int s = 0; s < TILE / 64; ++s) {
@@ -537,11 +597,7 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
         for (int z = 0; z < 4; ++z) slab[i * LD + j + z] = v[z];
       }
       if (PHASE == PHASE_LAST) {
-        if (!tall && i0 + i < it.rows) {
-#pragma unroll
-          for (int z = 0; z < 4; ++z)
-            if (j0 + j + z < it.cols) put(i0 + i, j0 + j + z, v[z]);
-        }
+        if (!tall) put(i0 + i, j0 + j, v);
       } else {
         split_n<4>(v, (_Float16*)&hi, (_Float16*)&lo);
         const int64_t d = at<W>(i0 + i, L.rp, j0 + j);
@@ -564,11 +620,8 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
 #pragma unroll
       for (int z = 0; z < 8; ++z) v[z] = slab[(i + z) * LD + j];
       if (PHASE == PHASE_LAST) {
-        if (j0 + j < it.rows) {
-#pragma unroll
-          for (int z = 0; z < 8; ++z)
-            if (i0 + i + z < it.cols) put(j0 + j, i0 + i + z, v[z]);
-        }
+        put(j0 + j, i0 + i, v);
+        put(j0 + j, i0 + i + 4, v + 4);
       } else {
         half8 hi, lo;
         split_n<8>(v, (_Float16*)&hi, (_Float16*)&lo);
