@@ -471,6 +471,14 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
     own(i, j, own_hi[o], own_lo[o]);
   }
 
+  // hi lo + lo hi on their own where registers allow it: a matrix instruction rounds its sum each time, and these are
+  // 2^-11 of hi hi (the renderer's matrices: 0.5 of float32 products' error, 0.7 in one sum)
+  constexpr bool APART = W == 2 && TILE == 64;
+  floatx4 cross[APART ? FM : 1][APART ? FN : 1];
+#pragma unroll
+  for (int i = 0; i < (APART ? FM : 1); ++i)
+#pragma unroll
+    for (int j = 0; j < (APART ? FN : 1); ++j) cross[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
   const int frow = lane & 15;
   for (int s = 0; s < NBUF - 1 && s < stages; ++s) issue(s);
   const int fchunk = ((lane >> 4) ^ (lane & 7)) << 4;
@@ -495,18 +503,26 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
 #pragma unroll
       for (int j = 0; j < FN; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0[i], b0[j], acc[i][j], 0, 0, 0);
-    if (W == 2) {
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0[i], b1[j], acc[i][j], 0, 0, 0);
-    }
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1[i], W == 2 ? b0[j] : b1[j], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < FN; ++j) {
+        floatx4& to = APART ? cross[APART ? i : 0][APART ? j : 0] : acc[i][j];
+        if (W == 2) to = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0[i], b1[j], to, 0, 0, 0);
+      }
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        floatx4& to = APART ? cross[APART ? i : 0][APART ? j : 0] : acc[i][j];
+        to = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1[i], W == 2 ? b0[j] : b1[j], to, 0, 0, 0);
+      }
+  }
+  if (APART) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] += cross[APART ? i : 0][APART ? j : 0];
   }
   __syncthreads();
 
