@@ -308,7 +308,7 @@ def newton_schulz(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float
     iteration of torch.optim.Muon.
 
     ``mats``: a tensor [..., rows, cols] (a stack of matrices) or a list of such; float32 or bfloat16; returns the
-    same structure, contiguous.  ``prec``: 0 fp32's accuracy (float32's default), 1 bfloat16's (its default).  A zero
+    same structure, contiguous and without autograd history.  ``prec``: 0 fp32's accuracy (float32's default), 1 bfloat16's (its default).  A zero
     matrix gives zeros, one with NaN or infinities NaN.  All matrices share the same few launches."""
     if isinstance(mats, torch.Tensor):
         return newton_schulz([mats], steps, coefficients, eps, prec)[0]
@@ -372,6 +372,8 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
         if t is not None and (t.dtype != torch.float32 or t.numel() < k or not t.is_contiguous()
                               or t.device != params[0].device):
             raise ValueError("muon_step: sumsq and hyper are contiguous float32 on the weights' device")
+    if sumsq is not None and not max_norm > 0.0:
+        raise ValueError(f"muon_step: clipping by sumsq needs a positive max_norm, got {max_norm}")
     a, b, c = (float(x) for x in coefficients)
     for dtype, bf16 in _MATRIX_DTYPES.items():
         pick = [i for i, p in enumerate(params) if p.dtype == dtype]

@@ -268,3 +268,34 @@ def test_another_stream(dev, gen):
     torch.cuda.synchronize()
     for o in outs + here:
         assert torch.equal(o, want)
+
+
+def test_refusals(dev):
+    from multimodalstudio_amd import hip_ops
+    p, m = torch.zeros(6, 8, device="cuda"), torch.zeros(6, 8, device="cuda")
+    for bad in (lambda: hip_ops.newton_schulz(p.half()), lambda: hip_ops.newton_schulz([p, p.double()]),
+                lambda: hip_ops.muon_step([p.half()], [p.half()], [m], lr=0.1)):
+        with pytest.raises(TypeError):
+            bad()
+    s = torch.ones(1, device="cuda")
+    for bad in (lambda: hip_ops.newton_schulz(p[0]), lambda: hip_ops.muon_step([p], [p[:5]], [m], lr=0.1),
+                lambda: hip_ops.muon_step([p], [p], [m[:, :4]], lr=0.1),
+                lambda: hip_ops.muon_step([p], [p.bfloat16()], [m], lr=0.1),
+                lambda: hip_ops.muon_step([p], [p], [m.bfloat16()], lr=0.1),
+                lambda: hip_ops.muon_step([p], [p], [torch.zeros(8, 6, device="cuda").mT], lr=0.1),
+                lambda: hip_ops.muon_step([torch.zeros(8, 6, device="cuda").mT], [p], [m], lr=0.1),
+                lambda: hip_ops.muon_step([p[:1].expand(6, 8)], [p], [m], lr=0.1),
+                lambda: hip_ops.muon_step([p, p], [p, p], [m, m.clone()], lr=0.1),
+                lambda: hip_ops.muon_step([p, p.clone()], [p, p], [m, m], lr=0.1),
+                lambda: hip_ops.muon_step([p], [p], [m], lr=0.1, sumsq=s),
+                lambda: hip_ops.muon_step([p], [p], [m], lr=0.1, sumsq=s.double(), max_norm=1.0),
+                lambda: hip_ops.muon_step([p], [p], [m], lr=0.1, hyper=s),
+                lambda: hip_ops.muon_step([p], [p], [m], lr=0.1, adjust="none")):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: hip_ops.newton_schulz(p, steps=0), lambda: hip_ops.newton_schulz(p, eps=0.0),
+                lambda: hip_ops.newton_schulz(p, prec=3), lambda: hip_ops.newton_schulz(p.cpu()),
+                lambda: hip_ops.muon_step([p], [p], [m], lr=0.1, momentum=1.0)):
+        with pytest.raises(RuntimeError):
+            bad()
+    assert (p == 0).all() and (m == 0).all()
