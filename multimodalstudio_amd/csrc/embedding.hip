@@ -32,10 +32,18 @@ __device__ __forceinline__ Piece<T> load_piece(const T* p, int count) {
   }
   return x;
 }
-template <bool WHOLE, typename T>
+// STREAM: past the caches, for an output that is larger than they are
+typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(2)));
+template <bool WHOLE, bool STREAM = false, typename T>
 __device__ __forceinline__ void store_piece(T* p, const Piece<T>& x, int count) {
   if (WHOLE || count >= Piece<T>::N) {
-    __builtin_memcpy(p, &x, 16);
+    if (STREAM) {
+      words4 w;
+      __builtin_memcpy(&w, &x, 16);
+      __builtin_nontemporal_store(w, (words4*)p);
+    } else {
+      __builtin_memcpy(p, &x, 16);
+    }
   } else {
 #pragma unroll
     for (int q = 0; q < Piece<T>::N; ++q)
@@ -88,7 +96,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(Ids I, int64_t n, co
       asm("" : "+v"(y));   // rounded to fp32 before fp16 (not v_fma_mixlo's one rounding): the bits of the same product in torch
       x[r].v[q] = (T)y;
     }
-    store_piece<WHOLE>(out + (i0 + r) * ldo + c, x[r], dim - c);
+    store_piece<WHOLE, (R > 1)>(out + (i0 + r) * ldo + c, x[r], dim - c);
   }
 }
 
@@ -100,6 +108,7 @@ struct Zeros {
   int64_t rows;         // rows of `bytes` bytes, `ld` apart
   int64_t bytes, ld;
   int first;            // the launch's first block that clears
+  int stream;           // past the caches: a table that is larger than half of the last one's 256 MB
 };
 constexpr int64_t kZeroChunk = 1 << 16;   // bytes per such block
 
@@ -113,9 +122,12 @@ __device__ __forceinline__ bool clear_rows(const Zeros& Z) {
   for (int64_t e = begin + threadIdx.x; e < end; e += blockDim.x) {
     const int64_t r = dense ? 0 : e / per, c = (e - r * per) * 16;
     char* p = Z.p + r * Z.ld + c;
-    if (c + 16 <= bytes) __builtin_memcpy(p, &zero, 16);
-    else
+    if (c + 16 > bytes)
       for (int64_t b = c; b < bytes; b += 2, p += 2) *(uint16_t*)p = 0;
+    else if (Z.stream)
+      __builtin_nontemporal_store(words4{0, 0, 0, 0}, (words4*)p);
+    else
+      __builtin_memcpy(p, &zero, 16);
   }
   return true;
 }
@@ -681,7 +693,8 @@ template <typename T>
 void launch_fwd(const Ids& I, int64_t n, const void* table, int64_t ldt, int dim, float scale, void* out, int64_t ldo,
                 hipStream_t s) {
   constexpr int N = Piece<T>::N;
-  // 4 rows a team once there are blocks enough
+  // 4 rows a team, past the caches, once there are blocks enough (33 MB of output; 16384 x 4096 bf16: 46 us with one row
+  // a team, 42 with 4, 32 past the caches)
   const int l = lanes_for(dim, N), segs = (dim + (N << l) - 1) / (N << l);
   const bool many = (n << l) * segs >= 4 * 256 * 2048;
   const int per = (256 >> l) * (many ? 4 : 1);
@@ -771,7 +784,7 @@ MMS_EXPORT int mms_embedding_bwd(const void* ids, int ids64, int64_t ids_stride,
   const bool one = n <= kOneRounds * kSortThreads;
   // As much as hides in the sort's launches, in one of a single block or two for each digit (9001 indices below 50257, 771
   // wide: 70 us with nothing cleared there, 63 with 24 MB a launch, 56 with 48; 65536 below 131072, 2048 wide: 197, 192,
-  // 189, and 196 with 136 MB, all of the table).
+  // 189, and 196 with 136 MB, all of the table; past the caches 51 and 179).
   const int es = dtype == 0 ? 4 : 2, launches = one ? 1 : 2 * p.passes;
   const int64_t row_bytes = (int64_t)dim * es;
   const int64_t share = one ? ((n + kSortThreads - 1) / kSortThreads * p.passes * 5 + 10) << 20 : 48 << 20;
@@ -781,7 +794,7 @@ MMS_EXPORT int mms_embedding_bwd(const void* ids, int ids64, int64_t ids_stride,
   int64_t begun = 0;
   // the next launch's share of the rows, and its blocks behind `first` others
   const auto zeros = [&](int64_t first, unsigned& blocks) {
-    Zeros Z{(char*)dtable + begun * ldg * es, begun + each < cleared ? each : cleared - begun, row_bytes, ldg * es, (int)first};
+    Zeros Z{(char*)dtable + begun * ldg * es, begun + each < cleared ? each : cleared - begun, row_bytes, ldg * es, (int)first, rows * row_bytes > (128 << 20)};
     begun += Z.rows;
     const int64_t pieces = Z.ld == Z.bytes ? (Z.rows * Z.bytes + 15) / 16 : Z.rows * ((Z.bytes + 15) / 16);
     blocks = (unsigned)(first + (pieces + kZeroChunk / 16 - 1) / (kZeroChunk / 16));
