@@ -40,6 +40,8 @@ typedef MMS_GLOBAL char gchar;
 typedef MMS_GLOBAL _Float16 ghalf;
 typedef MMS_GLOBAL half4 ghalf4;
 typedef MMS_GLOBAL half8 ghalf8;
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4v lds_short4;
 
 constexpr int kMaxMatrices = 4096;       // (or stacks) per call
 constexpr int kNsItems = 48;             // matrices (or stacks of them) per launch: the argument struct stays < 4 KB
@@ -98,9 +100,8 @@ struct NsLayout {
     rp = (r + 63) / 64 * 64;
     cp = (c + 63) / 64 * 64;
   }
-  __host__ __device__ int64_t x() const { return kNormBlocks * (int64_t)sizeof(double); }
-  __host__ __device__ int64_t xt(int i) const { return x() + (int64_t)rp * cp * w * 2 * (1 + i); }
-  __host__ __device__ int64_t a() const { return x() + (int64_t)rp * cp * w * 6; }
+  __host__ __device__ int64_t x(int i) const { return kNormBlocks * (int64_t)sizeof(double) + (int64_t)rp * cp * w * 2 * i; }
+  __host__ __device__ int64_t a() const { return x(2); }
   __host__ __device__ int64_t b() const { return a() + (int64_t)rp * rp * w * 2; }
   __host__ __device__ int64_t xlo() const { return b() + (int64_t)rp * rp * w * 2; }
   __host__ __device__ int64_t bytes() const { return xlo() + (w == 1 ? (int64_t)rp * cp * 2 : 0); }
@@ -250,8 +251,8 @@ __device__ __forceinline__ void split_n(const float* v, _Float16* hi, _Float16* 
   }
 }
 
-// ---- X and X^T of u / |u| -----------------------------------------------------------------------------------------
-// One 64 x 64 tile of u per block through LDS, written in both orders; the rows and columns of the padding as zeros.
+// ---- X of u / |u| -------------------------------------------------------------------------------------------------
+// One 64 x 64 tile of u per block through LDS, written on the side with fewer rows; the padding as zeros.
 template <int W>
 __global__ __launch_bounds__(256) void ns_pack_kernel(const NsTable* __restrict__ T, NsStep S, int bf16) {
   __shared__ float t[64][65];
@@ -324,28 +325,19 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const NsTable* __restrict_
     t[i][quads ? lane16 * 4 + (e & 3) : lane64] = (float)(u * inv);
   }
   __syncthreads();
-  // the tile in its own order is X (wide) or X^T (tall); the other one gets the transposed tile
-  ghalf* X = (ghalf*)(ws + L.x());
-  ghalf* XT = (ghalf*)(ws + L.xt(0));
+  ghalf* X = (ghalf*)(ws + L.x(0));
   ghalf* Xlo = (ghalf*)(ws + L.xlo());
-  ghalf* same = tall ? XT : X;
-  ghalf* other = tall ? X : XT;
-  const int rs = tall ? L.cp : L.rp, ro = tall ? L.rp : L.cp;
+  const int x0 = tall ? j0 : i0, y0 = tall ? i0 : j0;
   for (int e = threadIdx.x; e < 64 * 16; e += 256) {
     const int a = (e >> 3) & 63, b = (e >> 9) * 32 + (e & 7) * 4;   // 8 threads: the 32 columns of a row; then rows
     half4 hi, lo;
-    float v[4] = {t[a][b], t[a][b + 1], t[a][b + 2], t[a][b + 3]};
+    float v[4];
+#pragma unroll
+    for (int z = 0; z < 4; ++z) v[z] = tall ? t[b + z][a] : t[a][b + z];
     split_n<4>(v, (_Float16*)&hi, (_Float16*)&lo);
-    int64_t d = at<W>(i0 + a, rs, j0 + b);
-    *(ghalf4*)(same + d) = hi;
-    if (W == 2) *(ghalf4*)(same + d + 32) = lo;
-    else if (!tall) *(ghalf4*)(Xlo + d) = lo;
-    float u[4] = {t[b][a], t[b + 1][a], t[b + 2][a], t[b + 3][a]};
-    split_n<4>(u, (_Float16*)&hi, (_Float16*)&lo);
-    d = at<W>(j0 + a, ro, i0 + b);
-    *(ghalf4*)(other + d) = hi;
-    if (W == 2) *(ghalf4*)(other + d + 32) = lo;
-    else if (tall) *(ghalf4*)(Xlo + d) = lo;
+    const int64_t d = at<W>(x0 + a, L.rp, y0 + b);
+    *(ghalf4*)(X + d) = hi;
+    *(ghalf4*)(W == 2 ? X + d + 32 : Xlo + d) = lo;
   }
 }
 
@@ -368,6 +360,11 @@ __device__ __forceinline__ const char* uniform(const char* p) {
 // One TILE x TILE tile of P Q^T per block.  WM x WN: a wave's part.  A stage is 128 bytes of every row (64 values, or 32
 // hi and 32 lo), brought to LDS by DMA; the 16-byte chunk c of row i lies at c ^ (i & 7), which makes the fragment reads
 // (8 lanes = 8 rows, one chunk) free of bank conflicts.  NBUF stages form a ring, NBUF - 1 of them in flight.
+//
+// The product with X has X's rows along k: a stage of it is 64 (32) rows of the tile's columns, 4 KB for each 32 columns,
+// and its fragments are read by the transposing LDS loads: 16 lanes read 4 rows of 16 columns, and each gets one column
+// of them.  There a row's 32-byte piece lies at piece ^ f(row), f by bit 3 of the row (and bit 1 where rows are 128
+// bytes): the 8 rows that 32 lanes read are in different banks.  So X^T is kept nowhere.
 template <int TILE, int WM, int WN, int NBUF, int W, int PHASE>
 __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_kernel(
     const NsTable* __restrict__ T, NsStep S, float ca, float cb, float cc, int parity, int bf16) {
@@ -406,8 +403,8 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
     tj = in / h;
   }
   gchar* ws = (gchar*)it.ws + k * L.bytes();
-  const ghalf* P = (const ghalf*)(ws + (PHASE == PHASE_A ? L.x() : PHASE == PHASE_B ? L.a() : L.b()));
-  const ghalf* Q = PHASE <= PHASE_B ? P : (const ghalf*)(ws + L.xt(parity));
+  const ghalf* P = (const ghalf*)(ws + (PHASE == PHASE_A ? L.x(parity) : PHASE == PHASE_B ? L.a() : L.b()));
+  const ghalf* Q = PHASE <= PHASE_B ? P : (const ghalf*)(ws + L.x(parity));
   const int K = PHASE == PHASE_A ? L.cp : L.rp;
   const int qrows = PHASE <= PHASE_B ? L.rp : L.cp;
   const int stages = __builtin_amdgcn_readfirstlane(K * W / 64);
@@ -423,23 +420,31 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
   for (int l = 0; l < LOADS; ++l) {
     const int part = 8 * (l * NW + wave), row = part % TILE, row0 = (part < TILE ? ti : tj) * TILE;
     const int left = (part < TILE ? L.rp : qrows) - row0;
-    src[l] = uniform((const char*)(part < TILE ? P : Q) + (int64_t)(row0 + (row < left ? row : 0)) * (64 * W));
+    const int row1 = row0 + (row < left ? row : 0);
+    if (PHASE >= PHASE_X && part >= TILE)   // 32 columns: 4 instructions
+      src[l] = uniform((const char*)Q + (int64_t)(row1 >> 5) * L.rp * (64 * W) + (row >> 3 & 3) * 1024);
+    else
+      src[l] = uniform((const char*)(part < TILE ? P : Q) + (int64_t)row1 * (64 * W));
   }
   // the lane's chunk; in prec 1 a stage's row is two of the operand's 64-byte ones
   const int lrow = lane >> 3, lchunk = (lane & 7) ^ lrow;
   const uint32_t off = lrow * (64 * W) + (W == 1 ? lchunk & 3 : lchunk) * 16;
   const uint32_t offp = off + (W == 1 ? (lchunk >> 2) * L.rp * 64 : 0);
-  const uint32_t offq = off + (W == 1 ? (lchunk >> 2) * qrows * 64 : 0);
+  uint32_t offq = off + (W == 1 ? (lchunk >> 2) * qrows * 64 : 0);
+  if (PHASE >= PHASE_X) {
+    const int f = W == 1 ? lane >> 5 : (lane >> 4 & 1) | (wave & 1) << 1;   // (an instruction's rows: 8 x its number)
+    offq = (lane ^ 2 * f) * 16;
+  }
   const auto issue = [&](int s) {
     const uint32_t dst = lds0 + (s % NBUF) * STAGE + wave * 1024;
-    const int64_t sp = (int64_t)s * L.rp * 128, sq = (int64_t)s * qrows * 128;
+    const int64_t sp = (int64_t)s * L.rp * 128, sq = PHASE >= PHASE_X ? (int64_t)s * 4096 : (int64_t)s * qrows * 128;
 #pragma unroll
     for (int l = 0; l < LOADS; ++l) {
       const bool p = 8 * (l * NW + wave) < TILE;
       lds_dma16_s(src[l] + (p ? sp : sq), p ? offp : offq, dst + l * NW * 1024);
     }
   };
-  static_assert(LOADS * NW * 8 == 2 * TILE, "whole instructions");
+  static_assert(LOADS * NW * 8 == 2 * TILE && NW % 2 == 0, "whole instructions");
 
   floatx4 acc[FM][FN];
 #pragma unroll
@@ -458,7 +463,7 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
   };
   const auto own = [&](int i, int j, half4& hi, half4& lo) {
     const int64_t d = at<W>(ti * TILE + i, L.rp, tj * TILE + j);
-    const ghalf* x = PHASE == PHASE_B ? P : (const ghalf*)(ws + L.x());
+    const ghalf* x = PHASE == PHASE_B ? P : (const ghalf*)(ws + L.x(parity));
     hi = *(const ghalf4*)(x + d);
     if (W == 2) lo = *(const ghalf4*)(x + d + 32);
     else if (PHASE >= PHASE_X) lo = *(const ghalf4*)((const ghalf*)(ws + L.xlo()) + d);
@@ -482,20 +487,43 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
   const int frow = lane & 15;
   for (int s = 0; s < NBUF - 1 && s < stages; ++s) issue(s);
   const int fchunk = ((lane >> 4) ^ (lane & 7)) << 4;
+  // the lane's place in the two halves of 32 columns of X's rows, and the distance from hi to lo or to the next 32 rows
+  int ftr[FN], fnext;
+  if (PHASE >= PHASE_X) {
+    const int g = lane >> 4, row = g * 8 + (frow >> 2), f = W == 1 ? g & 1 : (lane >> 3 & 1) | (g & 1) << 1;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int u = wn * FN + j;
+      ftr[j] = (u >> 1) * 4096 + row * (64 * W) + ((u & 1) ^ f) * 32 + (lane & 3) * 8;
+    }
+    fnext = W == 1 ? 2048 : 64 - (f >> 1) * 128;
+  }
+  const auto column = [&](const char* p) {   // 8 rows of a column: two reads of 4
+    half8 v;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const half4 x = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + h * 256 * W)));
+#pragma unroll
+      for (int z = 0; z < 4; ++z) v[h * 4 + z] = x[z];
+    }
+    return v;
+  };
   for (int s = 0; s < stages; ++s) {
     // stage s has arrived once only the loads issued after it are outstanding; all waves are then past stage s - 1
     if (s + NBUF - 2 < stages) wait_vm_barrier<(NBUF - 2) * LOADS>();
     else wait_vm_barrier<0>();
     if (s + NBUF - 1 < stages) issue(s + NBUF - 1);
     const char* pa = lds + (s % NBUF) * STAGE + (wm * WM + frow) * 128;
-    const char* pq = lds + (s % NBUF) * STAGE + (TILE + wn * WN + frow) * 128;
+    const char* pq = lds + (s % NBUF) * STAGE + (TILE + (PHASE >= PHASE_X ? 0 : wn * WN + frow)) * 128;
     half8 a0[FM], a1[FM], b0[FN], b1[FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i) a0[i] = *(const half8*)(pa + i * 2048 + fchunk);
 #pragma unroll
-    for (int j = 0; j < FN; ++j) b0[j] = *(const half8*)(pq + j * 2048 + fchunk);
+    for (int j = 0; j < FN; ++j)
+      b0[j] = PHASE >= PHASE_X ? column(pq + ftr[j]) : *(const half8*)(pq + j * 2048 + fchunk);
 #pragma unroll
-    for (int j = 0; j < FN; ++j) b1[j] = *(const half8*)(pq + j * 2048 + (fchunk ^ 64));
+    for (int j = 0; j < FN; ++j)
+      b1[j] = PHASE >= PHASE_X ? column(pq + ftr[j] + fnext) : *(const half8*)(pq + j * 2048 + (fchunk ^ 64));
 #pragma unroll
     for (int i = 0; i < FM; ++i) a1[i] = *(const half8*)(pa + i * 2048 + (fchunk ^ 64));
 #pragma unroll
@@ -529,8 +557,7 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
   // epilogue: 64 rows at a time through LDS in fp32 (odd row length: columns are read without conflicts too)
   constexpr int LD = TILE + 1;
   float* slab = (float*)lds;
-  ghalf* X = (ghalf*)(ws + L.x());
-  ghalf* XT = (ghalf*)(ws + L.xt(parity ^ 1));
+  ghalf* X = (ghalf*)(ws + L.x(parity ^ 1));
   ghalf* Xlo = (ghalf*)(ws + L.xlo());
   ghalf* D = (ghalf*)(ws + (PHASE == PHASE_A ? L.a() : L.b()));
   const bool tall = it.rows > it.cols;
@@ -608,7 +635,7 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
           v[z] = PHASE == PHASE_B ? __builtin_fmaf(cb, y, cc * v[z]) : __builtin_fmaf(ca, y, v[z]);
         }
       }
-      if (PHASE != PHASE_A) {
+      if (PHASE == PHASE_B || PHASE == PHASE_LAST) {
 #pragma unroll
         for (int z = 0; z < 4; ++z) slab[i * LD + j + z] = v[z];
       }
@@ -623,8 +650,8 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
         else if (PHASE == PHASE_X) *(ghalf4*)(Xlo + d) = lo;
       }
     }
-    // the other order: X^T, the mirrored triangle, or a tall result
-    if (PHASE <= PHASE_B && ti == tj) continue;
+    // the other order: the mirrored triangle, or a tall result
+    if (PHASE == PHASE_X || (PHASE <= PHASE_B && ti == tj)) continue;
     if (PHASE == PHASE_LAST && !tall) continue;
     __syncthreads();
     for (int e = threadIdx.x; e < 64 * TILE / 8; e += NT) {
@@ -641,7 +668,7 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
       } else {
         half8 hi, lo;
         split_n<8>(v, (_Float16*)&hi, (_Float16*)&lo);
-        ghalf* d = (PHASE == PHASE_X ? XT : D) + at<W>(j0 + j, width, i0 + i);
+        ghalf* d = D + at<W>(j0 + j, width, i0 + i);
         *(ghalf8*)d = hi;
         if (W == 2) *(ghalf8*)(d + 32) = lo;
       }
