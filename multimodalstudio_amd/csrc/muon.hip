@@ -70,15 +70,18 @@ struct NsArgs {
 
 // The items again, in the workspace: written by the first launch, read by the others.  (Kernel arguments lie in host
 // memory: 3.6 KB of them cost each launch several us on the host, and each block a slow read.)
+constexpr int kMaxParts = 1024;   // blocks of a launch of A whose tiles are summed in parts
 struct NsTable {
   int blk0[4][64];          // first block of each item: packing, A, B, X; INT_MAX past the last
   NsItem it[kNsItems];
+  int arrived[kMaxParts];   // parts of a tile of A that are through; zero between launches
 };
-constexpr int64_t kTableBytes = 4608;
+constexpr int64_t kTableBytes = 8704;
 static_assert(sizeof(NsTable) <= kTableBytes, "the table's part of the workspace");
 enum { MAP_PACK = 0, MAP_A = 1, MAP_B = 2, MAP_X = 3 };
 struct NsTiles {
   int a, b, x;
+  int chunk;   // stages of A that a block sums, at most
 };
 
 struct NsStep {
@@ -145,6 +148,9 @@ __host__ __device__ inline int full_blocks(const NsLayout& L, int tile) {
   return ((L.rp + tile - 1) / tile) * ((L.cp + tile - 1) / tile);
 }
 
+// blocks that share the sum of a tile of A, each over `chunk` stages of 128 bytes along k
+__host__ __device__ inline int gram_parts(const NsLayout& L, int chunk) { return (L.cp * L.w / 64 + chunk - 1) / chunk; }
+
 __device__ __forceinline__ float load1(const MMS_GLOBAL void* p, int64_t i, bool bf16) {
   if (bf16) return __uint_as_float((uint32_t)((const MMS_GLOBAL uint16_t*)p)[i] << 16);
   return ((const MMS_GLOBAL float*)p)[i];
@@ -173,8 +179,8 @@ __global__ __launch_bounds__(256) void muon_momentum_kernel(NsArgs A, NsStep S, 
     const int i = threadIdx.x, k = i < A.n ? i : 0;
     const NsItem it = A.it[k];
     const NsLayout L(it.rows, it.cols, w);
-    const int count[4] = {pack_blocks(L) * it.batch, gram_blocks(L, tiles.a) * it.batch, gram_blocks(L, tiles.b) * it.batch,
-                          full_blocks(L, tiles.x) * it.batch};
+    const int count[4] = {pack_blocks(L) * it.batch, gram_blocks(L, tiles.a) * gram_parts(L, tiles.chunk) * it.batch,
+                          gram_blocks(L, tiles.b) * it.batch, full_blocks(L, tiles.x) * it.batch};
     for (int q = 0; q < 4; ++q) {
       int x = i < A.n ? count[q] : 0;
       for (int o = 1; o < 64; o <<= 1) {
@@ -185,6 +191,8 @@ __global__ __launch_bounds__(256) void muon_momentum_kernel(NsArgs A, NsStep S, 
     }
     if (i < A.n) table->it[i] = it;
   }
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < kMaxParts; i += 256) table->arrived[i] = 0;
   const int ii = find_item(A, blockIdx.x);
   const NsItem it = A.it[ii];
   const NsLayout L(it.rows, it.cols, w);
@@ -367,7 +375,8 @@ __device__ __forceinline__ const char* uniform(const char* p) {
 // bytes): the 8 rows that 32 lanes read are in different banks.  So X^T is kept nowhere.
 template <int TILE, int WM, int WN, int NBUF, int W, int PHASE>
 __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_kernel(
-    const NsTable* __restrict__ T, NsStep S, float ca, float cb, float cc, int parity, int bf16) {
+    NsTable* __restrict__ T, NsStep S, float ca, float cb, float cc, int parity, int bf16, int chunk,
+    uint64_t* __restrict__ partial) {
   constexpr int NWM = TILE / WM, NWN = TILE / WN, NW = NWM * NWN, NT = NW * 64;
   constexpr int STAGE = 2 * TILE * 128;          // bytes
   constexpr int LOADS = STAGE / (NW * 1024);     // DMA instructions per wave and stage, 8 rows each
@@ -379,7 +388,8 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
   const NsItem it = load_item(T, find_item(T, PHASE == PHASE_A ? MAP_A : PHASE == PHASE_B ? MAP_B : MAP_X, first));
   const NsLayout L(it.rows, it.cols, W);
   const int nr = (L.rp + TILE - 1) / TILE, nc = (L.cp + TILE - 1) / TILE;
-  const int per = PHASE <= PHASE_B ? nr * (nr + 1) / 2 : nr * nc;
+  const int tiles = PHASE <= PHASE_B ? nr * (nr + 1) / 2 : nr * nc;
+  const int parts = PHASE == PHASE_A ? __builtin_amdgcn_readfirstlane(gram_parts(L, chunk)) : 1, per = tiles * parts;
   int q = blockIdx.x - first, ti, tj;
   {
     // blocks b, b + 8, ... share an XCD: give each XCD a run of neighbouring tiles of the item
@@ -388,8 +398,10 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
     for (int y = 0; y < x; ++y) start += (last - y >= 0 ? ((last - y) >> 3) + 1 : 0) - (y < o ? 1 : 0);
     q = start + ((q + o) >> 3) - (x < o ? 1 : 0);
   }
-  const int k = q / per;
+  const int k = q / per, slot = first + q;
   q -= k * per;
+  const int part = PHASE == PHASE_A ? __builtin_amdgcn_readfirstlane(q / tiles) : 0;
+  q -= part * tiles;
   if (PHASE <= PHASE_B) {
     ti = (int)((sqrtf(8.f * q + 1.f) - 1.f) * 0.5f);
     while ((ti + 1) * (ti + 2) / 2 <= q) ++ti;
@@ -407,7 +419,8 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
   const ghalf* Q = PHASE <= PHASE_B ? P : (const ghalf*)(ws + L.x(parity));
   const int K = PHASE == PHASE_A ? L.cp : L.rp;
   const int qrows = PHASE <= PHASE_B ? L.rp : L.cp;
-  const int stages = __builtin_amdgcn_readfirstlane(K * W / 64);
+  const int stage0 = part * chunk, left = K * W / 64 - stage0;
+  const int stages = __builtin_amdgcn_readfirstlane(PHASE == PHASE_A && left > chunk ? chunk : left);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / NWN, wn = wave % NWN;
@@ -418,13 +431,14 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
   const char* src[LOADS];
 #pragma unroll
   for (int l = 0; l < LOADS; ++l) {
-    const int part = 8 * (l * NW + wave), row = part % TILE, row0 = (part < TILE ? ti : tj) * TILE;
-    const int left = (part < TILE ? L.rp : qrows) - row0;
-    const int row1 = row0 + (row < left ? row : 0);
-    if (PHASE >= PHASE_X && part >= TILE)   // 32 columns: 4 instructions
+    const int any = 8 * (l * NW + wave), row = any % TILE, row0 = (any < TILE ? ti : tj) * TILE;
+    const int rows = (any < TILE ? L.rp : qrows) - row0;
+    const int row1 = row0 + (row < rows ? row : 0);
+    if (PHASE >= PHASE_X && any >= TILE)   // 32 columns: 4 instructions
       src[l] = uniform((const char*)Q + (int64_t)(row1 >> 5) * L.rp * (64 * W) + (row >> 3 & 3) * 1024);
     else
-      src[l] = uniform((const char*)(part < TILE ? P : Q) + (int64_t)row1 * (64 * W));
+      src[l] = uniform((const char*)(any < TILE ? P : Q) + (int64_t)row1 * (64 * W) +
+                       (PHASE == PHASE_A ? (int64_t)stage0 * L.rp * 128 : 0));
   }
   // the lane's chunk; in prec 1 a stage's row is two of the operand's 64-byte ones
   const int lrow = lane >> 3, lchunk = (lane & 7) ^ lrow;
@@ -553,6 +567,49 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
       for (int j = 0; j < FN; ++j) acc[i][j] += cross[APART ? i : 0][APART ? j : 0];
   }
   __syncthreads();
+  if (PHASE == PHASE_A && parts > 1) {
+    // The sums of a tile in parts: each block leaves its own, the last one to arrive adds them all in their order (which
+    // block that is changes nothing) and goes on.  Nobody waits.  Blocks on different XCDs see each other's parts by
+    // loads and stores past their L2s (agent scope, 8 bytes each): a fence at that scope in their place writes back all
+    // of an L2, for each wave (300 x 4096 in 11 parts: 33 us with fences, 14 so).
+    constexpr int EACH = TILE * TILE / 2;
+    typedef uint64_t pair2 __attribute__((ext_vector_type(2)));
+    uint64_t* to = partial + (int64_t)slot * EACH + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const pair2 v = __builtin_bit_cast(pair2, acc[i][j]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          __hip_atomic_store(to + ((i * FN + j) * 2 + h) * NT, v[h], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // they are in memory
+    __syncthreads();
+    int* arrived = T->arrived + (slot - part * tiles);
+    if (threadIdx.x == 0)
+      *(int*)lds = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (__builtin_amdgcn_readfirstlane(*(const int*)lds) != parts - 1) return;
+    asm volatile("" ::: "memory");
+    if (threadIdx.x == 0) *arrived = 0;   // for the next step's launch
+    uint64_t* from = partial + (int64_t)(slot - part * tiles) * EACH + threadIdx.x;
+    for (int p = 0; p < parts; ++p) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          pair2 v;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            v[h] = __hip_atomic_load(from + ((i * FN + j) * 2 + h) * NT, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          const floatx4 x = __builtin_bit_cast(floatx4, v);
+          acc[i][j] = p ? acc[i][j] + x : x;
+        }
+      from += (int64_t)tiles * EACH;
+    }
+    __syncthreads();   // lds: the flag was read
+  }
 
   // epilogue: 64 rows at a time through LDS in fp32 (odd row length: columns are read without conflicts too)
   constexpr int LD = TILE + 1;
@@ -681,10 +738,11 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
 int width_of(int64_t rows, int64_t cols, int prec) { return prec == 0 || rows <= 128 || cols <= 128 ? 2 : 1; }
 
 // The launches of the matrices that share one table
-struct NsGroup {
-  NsArgs A;
-  int64_t norm, pack, a, b, x;   // blocks
+struct NsPlan {
+  int n, w;                            // matrices (or stacks), operands' width
+  int64_t norm, pack, a, b, x;         // blocks
   NsTiles tiles;
+  int64_t partial;                     // bytes of A's parts
 };
 
 // The tile of a launch whose item i has `count(i, t)` tiles of `stages(i)` stages: the one whose last block should end
@@ -692,26 +750,55 @@ struct NsGroup {
 // the end is neither before the n-th longest block had its turn on one of 256 CUs nor before the average CU is through.
 // Costs in us, from launches that fill the card: 64-wide tiles are bound by LDS reads, 128 by those and by products,
 // 192 and 256 by power (the clock falls to 1.6 GHz under 256-wide tiles, 1.2 PFLOP/s of fp16).  4096 x 4096, prec 1: A
-// 144, 109, 84, 104 us with 64, 128, 192, 256-wide tiles (253 of the 192-wide ones: one for each CU), X 229, 156, 178,
-// 136; six of 701 x 1100, prec 0: A 20, 28, 46, 70 us.
-constexpr int kTiles[4] = {256, 192, 128, 64};
-constexpr float kStageCost[2][4] = {{1.90f, 1.22f, 0.55f, 0.23f}, {2.25f, 1.40f, 0.78f, 0.26f}};
+// 158, 110, 87, 108 us with 64, 128, 192, 256-wide tiles (253 of the 192-wide ones: one for each CU), X 232, 163, 194,
+// 138; six of 701 x 1100, prec 0: A 20, 28, 46, 68 us, X 32, 33, 40, 54.
+// With `chunk`, tiles may be summed in parts of that many stages: as few parts as fill the card with one round of
+// blocks, and no more than the square root of the stages (a stage takes about as long as the adding of a part), where
+// that beats whole sums.  Parts cost 2 us, for their way through memory, and 0.3 for each that the last block adds.
+// prec 0: 64 x 4096 (128 stages) 38 us whole, 13 in 11 parts; 100 x 20000 (626) 177, 22 in 25 parts (29 in 53);
+// 300 x 4096 with 60 x 2000 and 1000 x 1000 40, 17.
+constexpr int kTiles[4] = {256, 192, 128, 64}, kPerCu[4] = {1, 1, 2, 3};
+constexpr float kGramCost[2][4] = {{1.90f, 1.22f, 0.55f, 0.23f}, {2.25f, 1.40f, 0.73f, 0.26f}};
+constexpr float kFullCost[2][4] = {{1.90f, 1.38f, 0.60f, 0.22f}, {2.00f, 1.38f, 0.62f, 0.21f}};
+constexpr int kMinChunk = 12;
 template <typename Count, typename Stages>
-int choose_tile(int n, int w, const Count& count, const Stages& stages) {
+int choose_tile(int n, const float (&cost)[4], const Count& count, const Stages& stages, int* chunk) {
   int best = 64;
-  float least = 0.f;
+  float least = 1e30f;
   for (int k = 0; k < 4; ++k) {
-    int64_t before = 0;
-    float sum = 0.f, end = 0.f;
-    for (int i = 0; i < n; ++i) {
-      const float each = kStageCost[w - 1][k] * (8 + stages(i));
-      const int64_t c = count(i, kTiles[k]);
-      before += c;
-      sum += each * c;
-      end = fmaxf(end, each * ((before + 255) / 256));
+    int64_t total = 0;
+    int longest = 0;
+    for (int whole = 1; whole >= (chunk ? 0 : 1); --whole) {
+      int len = 1 << 30;
+      if (!whole) {
+        // the longest sum in equal parts, the others in parts of the same length
+        const int64_t fill = (total + 256 * kPerCu[k] - 1) / (256 * kPerCu[k]);
+        const int least_len = std::max(kMinChunk, (int)sqrtf((float)longest));
+        const int l = (int)std::min<int64_t>(std::max<int64_t>(fill, least_len), longest);
+        const int parts = (longest + l - 1) / l;
+        if (parts < 2) break;
+        len = (longest + parts - 1) / parts;
+      }
+      int64_t before = 0;
+      float sum = 0.f, end = 0.f;
+      for (int i = 0; i < n; ++i) {
+        const int s = stages(i), parts = (int)(((int64_t)s + len - 1) / len);
+        const int64_t c = count(i, kTiles[k]) * parts;
+        const float each = cost[k] * (8 + std::min(s, len)) + (parts > 1 ? 2.f + 0.3f * parts * (kTiles[k] / 64) * (kTiles[k] / 64) : 0.f);
+        before += c;
+        sum += each * c;
+        end = fmaxf(end, each * ((before + 255) / 256));
+        total += whole ? c * s : 0;
+        longest = s > longest ? s : longest;
+      }
+      end = fmaxf(end, sum / 256);
+      if (!whole && before > kMaxParts) continue;
+      if (end < least) {
+        least = end;
+        best = kTiles[k];
+        if (chunk) *chunk = len;
+      }
     }
-    end = fmaxf(end, sum / 256);
-    if (k == 0 || end < least) { least = end; best = kTiles[k]; }
   }
   return best;
 }
@@ -728,13 +815,74 @@ int ns_check(const char* fn, int n, const int64_t* batch, const int64_t* rows, c
   return 0;
 }
 
+// The plan of the next matrices of `order` that one table holds: the first ones, as long as they have one width
+NsPlan plan_group(const int* order, int live, const int64_t* batch, const int64_t* rows, const int64_t* cols, int prec) {
+  NsPlan P{};
+  P.w = width_of(rows[order[0]], cols[order[0]], prec);
+  const auto layout = [&](int i) { return NsLayout((int)rows[order[i]], (int)cols[order[i]], P.w); };
+  for (; P.n < live && P.n < kNsItems; ++P.n) {
+    const int i = order[P.n];
+    if (width_of(rows[i], cols[i], prec) != P.w) break;
+    const int64_t norm = batch[i] * norm_blocks(rows[i], cols[i]), pack = batch[i] * pack_blocks(layout(P.n));
+    if (P.n && (P.norm + norm > kMaxBlocks || P.pack + pack > kMaxBlocks)) break;
+    P.norm += norm;
+    P.pack += pack;
+  }
+  const auto gram = [&](int i, int t) { return gram_blocks(layout(i), t) * batch[order[i]]; };
+  const auto full = [&](int i, int t) { return full_blocks(layout(i), t) * batch[order[i]]; };
+  const auto along = [&](int i) { return layout(i).cp * P.w / 64; };
+  const auto across = [&](int i) { return layout(i).rp * P.w / 64; };
+  P.tiles.a = choose_tile(P.n, kGramCost[P.w - 1], gram, along, &P.tiles.chunk);
+  P.tiles.b = choose_tile(P.n, kGramCost[P.w - 1], gram, across, nullptr);
+  P.tiles.x = choose_tile(P.n, kFullCost[P.w - 1], full, across, nullptr);
+  bool split = false;
+  for (int i = 0; i < P.n; ++i) {
+    const int parts = gram_parts(layout(i), P.tiles.chunk);
+    split = split || parts > 1;
+    P.a += gram(i, P.tiles.a) * parts;
+    P.b += gram(i, P.tiles.b);
+    P.x += full(i, P.tiles.x);
+  }
+  P.partial = split ? P.a * P.tiles.a * P.tiles.a * (int64_t)sizeof(float) : 0;
+  return P;
+}
+
+// The matrices that are not empty, by width, largest first: their blocks are started first
+int sort_matrices(int n, const int64_t* batch, const int64_t* rows, const int64_t* cols, int prec, int* order) {
+  int live = 0;
+  for (int i = 0; i < n; ++i)
+    if (batch[i] * rows[i] * cols[i] > 0) order[live++] = i;
+  std::sort(order, order + live, [&](int i, int j) {
+    const int v = width_of(rows[i], cols[i], prec), w = width_of(rows[j], cols[j], prec);
+    const int64_t x = rows[i] + cols[i], y = rows[j] + cols[j];
+    return v != w ? v < w : x != y ? x > y : i < j;
+  });
+  return live;
+}
+
+// The workspace: A's parts, which the groups use in turn (`partial` bytes), then each group's table and operands.
+int64_t workspace_of(const int* order, int live, const int64_t* batch, const int64_t* rows, const int64_t* cols, int prec,
+                     NsPlan& first, int64_t& partial) {
+  int64_t bytes = 0;
+  partial = 0;
+  for (int at = 0; at < live;) {
+    const NsPlan P = plan_group(order + at, live - at, batch, rows, cols, prec);
+    if (at == 0) first = P;
+    bytes += kTableBytes;
+    for (int i = 0; i < P.n; ++i, ++at)
+      bytes += batch[order[at]] * NsLayout((int)rows[order[at]], (int)cols[order[at]], P.w).bytes();
+    partial = P.partial > partial ? P.partial : partial;
+  }
+  return bytes + partial;
+}
+
 template <int W, int PHASE>
-void launch_product(int tile, const NsTable* T, int64_t blocks, const NsStep& S, float a, float b, float c, int parity,
-                    int bf16, hipStream_t s) {
+void launch_product(int tile, NsTable* T, int64_t blocks, const NsStep& S, float a, float b, float c, int parity,
+                    int bf16, int chunk, uint64_t* partial, hipStream_t s) {
   const dim3 grid((unsigned)blocks);
 #define NS_LAUNCH(TILE, WM, WN, NBUF)                                                                            \
   hipLaunchKernelGGL((ns_product_kernel<TILE, WM, WN, NBUF, W, PHASE>), grid, dim3((TILE / WM) * (TILE / WN) * 64), 0, \
-                     s, T, S, a, b, c, parity, bf16)
+                     s, T, S, a, b, c, parity, bf16, chunk, partial)
   // 16 waves a CU where registers and LDS allow it: 8-wave blocks of 128 two at a time (482 us against 494 with 4 waves,
   // X of muon's four 2048 x 2048 and two 2048 x 5632 in prec 0), 16 of 64 x 64 rather than 8 of 128 x 64 for 256 (483,
   // 509), 4-wave blocks of 64 three at a time
@@ -746,15 +894,15 @@ void launch_product(int tile, const NsTable* T, int64_t blocks, const NsStep& S,
 }
 
 template <int W>
-void launch_group(const NsGroup& G, NsTable* T, const NsStep& S, int steps, float a, float b, float c, int bf16,
-                  hipStream_t s) {
-  hipLaunchKernelGGL(muon_momentum_kernel, dim3((unsigned)G.norm), dim3(256), 0, s, G.A, S, bf16, W, G.tiles, T);
-  hipLaunchKernelGGL((ns_pack_kernel<W>), dim3((unsigned)G.pack), dim3(256), 0, s, T, S, bf16);
+void launch_group(const NsPlan& P, const NsArgs& A, NsTable* T, const NsStep& S, int steps, float a, float b, float c,
+                  int bf16, uint64_t* partial, hipStream_t s) {
+  hipLaunchKernelGGL(muon_momentum_kernel, dim3((unsigned)P.norm), dim3(256), 0, s, A, S, bf16, W, P.tiles, T);
+  hipLaunchKernelGGL((ns_pack_kernel<W>), dim3((unsigned)P.pack), dim3(256), 0, s, T, S, bf16);
   for (int i = 0; i < steps; ++i) {
-    launch_product<W, PHASE_A>(G.tiles.a, T, G.a, S, a, b, c, i & 1, bf16, s);
-    launch_product<W, PHASE_B>(G.tiles.b, T, G.b, S, a, b, c, i & 1, bf16, s);
-    if (i + 1 < steps) launch_product<W, PHASE_X>(G.tiles.x, T, G.x, S, a, b, c, i & 1, bf16, s);
-    else launch_product<W, PHASE_LAST>(G.tiles.x, T, G.x, S, a, b, c, i & 1, bf16, s);
+    launch_product<W, PHASE_A>(P.tiles.a, T, P.a, S, a, b, c, i & 1, bf16, P.tiles.chunk, partial, s);
+    launch_product<W, PHASE_B>(P.tiles.b, T, P.b, S, a, b, c, i & 1, bf16, 0, nullptr, s);
+    if (i + 1 < steps) launch_product<W, PHASE_X>(P.tiles.x, T, P.x, S, a, b, c, i & 1, bf16, 0, nullptr, s);
+    else launch_product<W, PHASE_LAST>(P.tiles.x, T, P.x, S, a, b, c, i & 1, bf16, 0, nullptr, s);
   }
 }
 
@@ -765,9 +913,13 @@ int ns_run(const char* fn, int n, const int64_t* batch, const int64_t* rows, con
   MMS_REQUIRE(steps >= 1 && steps <= 64, fn, "1 to 64 steps");
   MMS_REQUIRE(S.eps > 0.0, fn, "eps must be positive");
   MMS_REQUIRE(n == 0 || (p && ldp && bsp && g && ldg && bsg), fn, "null pointer table");
-  int64_t need = 0;
-  const int rc = mms_muon_workspace(n, batch, rows, cols, prec, &need);
+  const int rc = ns_check(fn, n, batch, rows, cols, prec);
   if (rc) return rc;
+  static thread_local int order[kMaxMatrices];
+  const int live = sort_matrices(n, batch, rows, cols, prec, order);
+  NsPlan P{};
+  int64_t parts = 0;
+  const int64_t need = workspace_of(order, live, batch, rows, cols, prec, P, parts);
   for (int i = 0; i < n; ++i) {
     if (batch[i] * rows[i] * cols[i] == 0) continue;
     MMS_REQUIRE(p[i] && g[i], fn, "null matrix");
@@ -779,54 +931,28 @@ int ns_run(const char* fn, int n, const int64_t* batch, const int64_t* rows, con
   MMS_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 255) == 0), fn,
               "workspace too small (mms_muon_workspace) or not 256-byte aligned");
   hipStream_t s = mms::as_stream(stream);
-  char* next = (char*)ws;
-  // largest first: their blocks are started first
-  static thread_local int order[kMaxMatrices];
-  int live = 0;
-  for (int i = 0; i < n; ++i)
-    if (batch[i] * rows[i] * cols[i] > 0) order[live++] = i;
-  std::sort(order, order + live, [&](int i, int j) {
-    const int64_t x = rows[i] + cols[i], y = rows[j] + cols[j];
-    return x != y ? x > y : i < j;
-  });
-  for (int w = 1; w <= 2; ++w) {
-    for (int at = 0; at < live;) {
-      // the next matrices that one table holds
-      NsGroup G{};
-      NsTable* T = (NsTable*)next;
-      for (; at < live && G.A.n < kNsItems; ++at) {
-        const int i = order[at];
-        if (width_of(rows[i], cols[i], prec) != w) continue;
-        const NsLayout L((int)rows[i], (int)cols[i], w);
-        const int64_t norm = batch[i] * norm_blocks(rows[i], cols[i]), pack = batch[i] * pack_blocks(L);
-        if (G.A.n && (G.norm + norm > kMaxBlocks || G.pack + pack > kMaxBlocks)) break;
-        if (G.A.n == 0) next += kTableBytes;
-        G.A.it[G.A.n] = NsItem{g[i], m ? m[i] : nullptr, p[i], next, bsg[i], bsp[i], (int)ldg[i], (int)ldp[i],
-                               (int)rows[i], (int)cols[i], (int)batch[i], scale ? scale[i] : 1.f};
-        G.A.blk0[G.A.n++] = (int)G.norm;
-        next += batch[i] * L.bytes();
-        G.norm += norm;
-        G.pack += pack;
-      }
-      if (G.A.n == 0) break;
-      G.A.blk0[G.A.n] = (int)G.norm;
-      const NsItem* it = G.A.it;
-      const auto layout = [&](int i) { return NsLayout(it[i].rows, it[i].cols, w); };
-      const auto gram = [&](int i, int t) { return (int64_t)gram_blocks(layout(i), t) * it[i].batch; };
-      const auto full = [&](int i, int t) { return (int64_t)full_blocks(layout(i), t) * it[i].batch; };
-      G.tiles.a = choose_tile(G.A.n, w, gram, [&](int i) { return layout(i).cp * w / 64; });
-      G.tiles.b = choose_tile(G.A.n, w, gram, [&](int i) { return layout(i).rp * w / 64; });
-      G.tiles.x = choose_tile(G.A.n, w, full, [&](int i) { return layout(i).rp * w / 64; });
-      for (int i = 0; i < G.A.n; ++i) {
-        G.a += gram(i, G.tiles.a);
-        G.b += gram(i, G.tiles.b);
-        G.x += full(i, G.tiles.x);
-      }
-      if (w == 1) launch_group<1>(G, T, S, steps, a, b, c, bf16, s);
-      else launch_group<2>(G, T, S, steps, a, b, c, bf16, s);
-      const int e = mms::check_launch(fn);
-      if (e) return e;
+  uint64_t* partial = (uint64_t*)ws;
+  char* next = (char*)ws + parts;
+  for (int at = 0; at < live;) {
+    if (at) P = plan_group(order + at, live - at, batch, rows, cols, prec);
+    NsTable* T = (NsTable*)next;
+    next += kTableBytes;
+    NsArgs A{};
+    A.n = P.n;
+    int64_t norm = 0;
+    for (int k = 0; k < P.n; ++k, ++at) {
+      const int i = order[at];
+      A.it[k] = NsItem{g[i], m ? m[i] : nullptr, p[i], next, bsg[i], bsp[i], (int)ldg[i], (int)ldp[i], (int)rows[i],
+                       (int)cols[i], (int)batch[i], scale ? scale[i] : 1.f};
+      A.blk0[k] = (int)norm;
+      next += batch[i] * NsLayout((int)rows[i], (int)cols[i], P.w).bytes();
+      norm += batch[i] * norm_blocks(rows[i], cols[i]);
     }
+    A.blk0[P.n] = (int)norm;
+    if (P.w == 1) launch_group<1>(P, A, T, S, steps, a, b, c, bf16, partial, s);
+    else launch_group<2>(P, A, T, S, steps, a, b, c, bf16, partial, s);
+    const int e = mms::check_launch(fn);
+    if (e) return e;
   }
   return 0;
 }
@@ -839,10 +965,10 @@ MMS_EXPORT int mms_muon_workspace(int n, const int64_t* batch, const int64_t* ro
   MMS_REQUIRE(bytes != nullptr, fn, "null output");
   const int rc = ns_check(fn, n, batch, rows, cols, prec);
   if (rc) return rc;
-  *bytes = 0;
-  for (int i = 0; i < n; ++i)
-    if (batch[i] * rows[i] * cols[i] > 0)
-      *bytes += kTableBytes + batch[i] * NsLayout((int)rows[i], (int)cols[i], width_of(rows[i], cols[i], prec)).bytes();
+  static thread_local int order[kMaxMatrices];
+  NsPlan first;
+  int64_t partial;
+  *bytes = workspace_of(order, sort_matrices(n, batch, rows, cols, prec, order), batch, rows, cols, prec, first, partial);
   return 0;
 }
 

@@ -36,11 +36,16 @@ def test_muon_workspace(L):
     assert _workspace(L, []) == (0, 0)
     assert _workspace(L, [(0, 4, 4), (1, 0, 9), (2, 7, 0)]) == (0, 0)
     rc, one = _workspace(L, [(1, 60, 100)])
-    # 64 x 128 padded: X, two X^T (hi and lo, 2 bytes each), A and A's polynomial 64 x 64, the norm's partial sums, the
-    # launches' table
-    assert rc == 0 and one - 4608 == 3 * 64 * 128 * 4 + 2 * 64 * 64 * 4 + 8192
+    # 64 x 128 padded: X and the next X (hi and lo, 2 bytes each), A and A's polynomial 64 x 64, the norm's partial sums,
+    # the launches' table
+    assert rc == 0 and one - 8704 == 2 * 64 * 128 * 4 + 2 * 64 * 64 * 4 + 8192
     assert _workspace(L, [(1, 100, 60)]) == (0, one)
-    assert _workspace(L, [(3, 60, 100)]) == (0, 4608 + 3 * (one - 4608))
+    assert _workspace(L, [(3, 60, 100)]) == (0, 8704 + 3 * (one - 8704))
+    # two matrices of one table; long rows: whole parts of 64 x 64 sums of A besides
+    assert _workspace(L, [(1, 60, 100), (1, 100, 60)]) == (0, 8704 + 2 * (one - 8704))
+    rc, long = _workspace(L, [(1, 60, 8192)])
+    parts = long - (8704 + 2 * 64 * 8192 * 4 + 2 * 64 * 64 * 4 + 8192)
+    assert rc == 0 and parts > 0 and parts % (64 * 64 * 4) == 0
     for shapes, word in (([(-1, 4, 4)], "sizes"), ([(1, 1 << 21, 4)], "sizes"), ([(1 << 20, 1 << 20, 1 << 20)], "sizes")):
         assert _workspace(L, shapes)[0] != 0 and word in _err(L)
     assert _workspace(L, [(1, 4, 4)], prec=2)[0] != 0 and "prec" in _err(L)

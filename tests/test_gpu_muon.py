@@ -74,6 +74,34 @@ def test_orthogonalisation(dev, gen, shape, dtype):
     assert torch.equal(out, hip_ops.newton_schulz(g))
 
 
+# sums over long rows are split over blocks: one tile and many, stacks, tall, beside short ones that are not split
+LONG = [[(1, 20000)], [(40, 5000)], [(4096, 17)], [(3, 130, 2100)], [(300, 4096)], [(700, 8192)], [(1024, 16384)],
+        [(60, 9000), (2000, 33), (50, 60), (3, 3), (2, 7, 3000)]]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shapes", LONG, ids=str)
+def test_long_rows(dev, gen, shapes, dtype):
+    from multimodalstudio_amd import hip_ops
+    mats = [gradient(s, gen, dtype) for s in shapes]
+    outs = hip_ops.newton_schulz(mats)
+    for g, out in zip(mats, outs):
+        want = iterate(g, torch.float64)
+        assert rel(out, want) <= tolerance(g, want), tuple(g.shape)
+    # whichever block adds a tile's parts: the same bits, in a replayed graph too
+    for _ in range(3):
+        assert all(torch.equal(x, y) for x, y in zip(outs, hip_ops.newton_schulz(mats)))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = hip_ops.newton_schulz(mats)
+    for _ in range(3):
+        for x in again:
+            x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(outs, again))
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 def test_many_matrices_in_one_call(dev, gen, dtype):
     """More matrices than one launch holds, of every tile size, with empty ones between them: each as if alone."""
