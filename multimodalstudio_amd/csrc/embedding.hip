@@ -10,6 +10,9 @@
 // further blocks of the same launch, but for the first rows, which the sort's launches clear beside their few blocks.
 #include "common.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace {
 
 typedef __bf16 bf16_t;
@@ -108,9 +111,10 @@ struct Zeros {
   int64_t rows;         // rows of `bytes` bytes, `ld` apart
   int64_t bytes, ld;
   int first;            // the launch's first block that clears
-  int stream;           // past the caches: a table that is larger than half of the last one's 256 MB
+  int stream;           // past the caches: a table of more than kLargeTable
 };
 constexpr int64_t kZeroChunk = 1 << 16;   // bytes per such block
+constexpr int64_t kLargeTable = 128 << 20;   // half of the last cache
 
 __device__ __forceinline__ bool clear_rows(const Zeros& Z) {
   if ((int)blockIdx.x < Z.first) return false;
@@ -633,6 +637,99 @@ __global__ __launch_bounds__(256) void few_join_kernel(Few F, T* __restrict__ dt
   }
 }
 
+// ---- few positions --------------------------------------------------------------------------------------------------
+// One launch and no workspace: every block reads all of the indices.  Blocks of teams sort them (each thread counts what
+// lies before its own) and a team per sorted position and column segment sums a row, if it begins there; further blocks
+// clear the rows of theirs that do not occur.  Launching bounds it (16 .. 128 positions: 8.5 us a call, 13 .. 16 with the
+// launches of a sort and of runs).  128 positions of one row, which one team sums: 13 .. 17 us, as with those; past that
+// it would be slower (256: 24).
+constexpr int kBriefN = 128, kBriefRows = 4096;
+
+struct Brief {
+  int n, dim, lanes_log2, accumulate;
+  float scale;
+  int row_blocks, zero_rows;   // blocks of teams, and rows that each of the others clears
+  int stream;
+};
+
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(256) void embedding_brief_kernel(Ids I, Brief B, const T* __restrict__ dout, int64_t ldd,
+                                                              T* __restrict__ dtable, int64_t ldg) {
+  constexpr int N = Piece<T>::N;
+  const int t = threadIdx.x;
+  const uint32_t mine = t < B.n ? key_at(I, t) : (uint32_t)I.rows;
+  const int c0 = (int)blockIdx.y * N << B.lanes_log2;
+  if ((int)blockIdx.x >= B.row_blocks) {
+    __shared__ bool present[kBriefRows];
+    const int64_t r0 = (int64_t)((int)blockIdx.x - B.row_blocks) * B.zero_rows;
+    const int nr = I.rows - r0 < B.zero_rows ? (int)(I.rows - r0) : B.zero_rows;
+    for (int r = t; r < nr; r += 256) present[r] = false;
+    __syncthreads();
+    if (mine >= r0 && mine < r0 + nr) present[mine - r0] = true;
+    __syncthreads();
+    const int c1 = min(B.dim, c0 + (N << B.lanes_log2)), per = (c1 - c0 + N - 1) / N;
+    for (int e = t; e < nr * per; e += 256) {
+      const int r = e / per, c = c0 + (e - r * per) * N;
+      if (present[r]) continue;
+      T* p = dtable + (r0 + r) * ldg + c;
+      if (B.stream) store_piece<WHOLE, true>(p, Piece<T>{}, c1 - c);
+      else store_piece<WHOLE>(p, Piece<T>{}, c1 - c);
+    }
+    return;
+  }
+  __shared__ uint4 key4[kBriefN / 4];
+  __shared__ uint32_t key[kBriefN];
+  __shared__ int pos[kBriefN], length[kBriefN];
+  if (t < kBriefN) ((uint32_t*)key4)[t] = mine;
+  __syncthreads();
+  int before = 0, same = 0;
+  for (int q = 0; q < B.n; q += 32) {   // (what is past n has the largest key)
+    uint4 k4[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) k4[u] = key4[q / 4 + u];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint32_t k[4] = {k4[u].x, k4[u].y, k4[u].z, k4[u].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        before += k[e] < mine || (k[e] == mine && q + 4 * u + e < t);
+        same += k[e] == mine;
+      }
+    }
+  }
+  if (t < B.n) {
+    key[before] = mine;
+    pos[before] = t;
+    length[before] = same;
+  }
+  __syncthreads();
+  const int team = t >> B.lanes_log2, i = (int)blockIdx.x * (256 >> B.lanes_log2) + team;
+  const int c = c0 + (t & ((1 << B.lanes_log2) - 1)) * N, left = B.dim - c;
+  if (i >= B.n || left <= 0) return;
+  const uint32_t row = key[i];
+  if (row >= I.rows || (i > 0 && key[i - 1] == row)) return;
+  const int end = i + length[i];
+  float acc[N];
+#pragma unroll
+  for (int q = 0; q < N; ++q) acc[q] = 0.f;
+  int at = i;
+  const auto some = [&](auto count) {   // rows loaded together
+    constexpr int U = decltype(count)::value;
+    Piece<T> x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = load_piece<WHOLE>(dout + (int64_t)pos[min(at + u, end - 1)] * ldd + c, left);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (at + u < end)
+#pragma unroll
+        for (int q = 0; q < N; ++q) acc[q] += (float)x[u].v[q];
+    at += U;
+  };
+  while (end - at > 8) some(std::integral_constant<int, 32>{});
+  while (at < end) some(std::integral_constant<int, 4>{});
+  put_row<T, WHOLE>(dtable + (int64_t)row * ldg + c, acc, B.scale, B.accumulate, left);
+}
+
 // ---- host ---------------------------------------------------------------------------------------------------------
 int piece_of(int dtype) { return dtype == 0 ? 4 : 8; }
 
@@ -652,7 +749,7 @@ int check_ids(const char* fn, const void* ids, int64_t stride, int64_t n, int64_
 }
 
 struct Plan {
-  bool few;
+  bool brief, few;
   int bits, passes, run, lanes_log2, part_ld;
   int64_t nblk, nruns, pairs, counts, part, total;   // byte offsets: the pairs' second buffer, ...
 };
@@ -663,6 +760,9 @@ Plan plan_for(int64_t n, int64_t rows, int dim, int dtype) {
   const int N = piece_of(dtype);
   p.lanes_log2 = lanes_for(dim, N);
   p.part_ld = (dim + N - 1) / N * N;
+  // Few positions: one launch.
+  p.brief = n > 0 && n <= kBriefN;
+  if (p.brief) return p;
   // Few rows: two launches instead of four to six, as long as the blocks' sums (rows of 256 positions) are less than the
   // positions themselves and a row's wave has no more than 64 blocks to add up.
   p.few = n > 0 && rows <= kFewRows && n <= 256 * kFewTile && dim <= 4096;
@@ -712,6 +812,19 @@ void launch_few(const Ids& I, const Few& F, const void* dout, int64_t ldd, void*
                      I, F, (const T*)dout, ldd);
   hipLaunchKernelGGL((few_join_kernel<T>), dim3((unsigned)F.rows, (unsigned)((F.dim + 63) / 64)), dim3(256), 0, s, F,
                      (T*)dtable, ldg);
+}
+
+template <typename T>
+void launch_brief(const Ids& I, Brief B, const void* dout, int64_t ldd, void* dtable, int64_t ldg, hipStream_t s) {
+  const int seg = Piece<T>::N << B.lanes_log2, teams = 256 >> B.lanes_log2;
+  B.row_blocks = (B.n + teams - 1) / teams;
+  const int64_t row = std::min(seg, B.dim) * (int64_t)sizeof(T);
+  B.zero_rows = (int)std::min<int64_t>(kBriefRows, std::max<int64_t>(1, kZeroChunk / row));
+  B.stream = I.rows * B.dim * (int64_t)sizeof(T) > kLargeTable;
+  const int64_t zeros = B.accumulate ? 0 : (I.rows + B.zero_rows - 1) / B.zero_rows;
+  const auto kernel = B.dim % Piece<T>::N == 0 ? embedding_brief_kernel<T, true> : embedding_brief_kernel<T, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(B.row_blocks + zeros), (unsigned)((B.dim + seg - 1) / seg)), dim3(256), 0, s,
+                     I, B, (const T*)dout, ldd, (T*)dtable, ldg);
 }
 
 template <typename T>
@@ -769,6 +882,13 @@ MMS_EXPORT int mms_embedding_bwd(const void* ids, int ids64, int64_t ids_stride,
   hipStream_t s = mms::as_stream(stream);
   const Ids I{ids, ids_stride, ids64, rows, padding_idx};
   char* w = (char*)ws;
+  if (p.brief) {
+    const Brief B{(int)n, dim, p.lanes_log2, accumulate, scale, 0, 0, 0};
+    if (dtype == 0) launch_brief<float>(I, B, dout, ldd, dtable, ldg, s);
+    else if (dtype == 1) launch_brief<bf16_t>(I, B, dout, ldd, dtable, ldg, s);
+    else launch_brief<_Float16>(I, B, dout, ldd, dtable, ldg, s);
+    return mms::check_launch(fn);
+  }
   if (p.few) {
     const Few F{n, (int)rows, dim, p.lanes_log2, accumulate, scale, p.nblk, (uint32_t*)w, (float*)(w + p.part), p.part_ld};
     if (dtype == 0) launch_few<float>(I, F, dout, ldd, dtable, ldg, s);
@@ -794,7 +914,8 @@ MMS_EXPORT int mms_embedding_bwd(const void* ids, int ids64, int64_t ids_stride,
   int64_t begun = 0;
   // the next launch's share of the rows, and its blocks behind `first` others
   const auto zeros = [&](int64_t first, unsigned& blocks) {
-    Zeros Z{(char*)dtable + begun * ldg * es, begun + each < cleared ? each : cleared - begun, row_bytes, ldg * es, (int)first, rows * row_bytes > (128 << 20)};
+    Zeros Z{(char*)dtable + begun * ldg * es, begun + each < cleared ? each : cleared - begun, row_bytes, ldg * es, (int)first,
+            rows * row_bytes > kLargeTable};
     begun += Z.rows;
     const int64_t pieces = Z.ld == Z.bytes ? (Z.rows * Z.bytes + 15) / 16 : Z.rows * ((Z.bytes + 15) / 16);
     blocks = (unsigned)(first + (pieces + kZeroChunk / 16 - 1) / (kZeroChunk / 16));

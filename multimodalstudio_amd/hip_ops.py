@@ -450,7 +450,7 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> tor
 def _embedding_workspace(n: int, rows: int, dim: int, dt: int) -> int:
     need = ctypes.c_int64(0)
     _lib.call("mms_embedding_bwd_workspace", n, rows, dim, dt, ctypes.addressof(need))
-    return max(1, need.value)
+    return need.value
 
 
 def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: float = 1.0,
@@ -483,10 +483,10 @@ def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: 
     n = ids.numel()
     need = _embedding_workspace(n, rows, dim, dt)
     with _on_device(dout):
-        ws = torch.empty(need, dtype=torch.uint8, device=dout.device)
+        ws = torch.empty(need, dtype=torch.uint8, device=dout.device) if need else None
         _lib.call("mms_embedding_bwd", flat.data_ptr(), ids.dtype is torch.int64, stride, n, d.data_ptr(),
                   dim if n <= 1 else d.stride(0), rows, dim, dt, scale, pad, out.data_ptr(),
-                  dim if rows == 1 else out.stride(0), bool(accumulate), ws.data_ptr(), need, _stream_of(dout))
+                  dim if rows == 1 else out.stride(0), bool(accumulate), _ptr(ws), need, _stream_of(dout))
     return out
 
 

@@ -92,7 +92,7 @@ def test_embedding_refusals(L):
         assert fwd(**kw) != 0 and word in _err(L), kw
     assert fwd(n=0, ids=None, table=None, out=None) == 0
 
-    def bwd(ids=4096, n=4, dout=4096, ldd=8, rows=5, dim=8, dtype=0, pad=-1, dtable=4096, ldg=8, acc=0, ws=4096,
+    def bwd(ids=4096, n=400, dout=4096, ldd=8, rows=5, dim=8, dtype=0, pad=-1, dtable=4096, ldg=8, acc=0, ws=4096,
             ws_bytes=1 << 40):
         return L.mms_embedding_bwd(ids, 1, 1, n, dout, ldd, rows, dim, dtype, 1.0, pad, dtable, ldg, acc, ws, ws_bytes,
                                    None)
@@ -106,7 +106,8 @@ def test_embedding_refusals(L):
     need = ctypes.c_int64(-1)
     assert L.mms_embedding_bwd_workspace(0, 5, 8, 0, ctypes.addressof(need)) == 0
     assert L.mms_embedding_bwd_workspace(1000, 5, 8, 0, None) != 0
-    # many rows: two lists of (row, position); few: a sum per row and 256 positions
+    # few positions: none; many rows: two lists of (row, position); few: a sum per row and 256 positions
+    assert L.mms_embedding_bwd_workspace(128, 500, 8, 0, ctypes.addressof(need)) == 0 and need.value == 0
     assert L.mms_embedding_bwd_workspace(1000, 500, 8, 0, ctypes.addressof(need)) == 0 and need.value > 2 * 8000
     assert L.mms_embedding_bwd_workspace(1000, 5, 8, 0, ctypes.addressof(need)) == 0 and need.value >= 4 * 5 * 8 * 4
 

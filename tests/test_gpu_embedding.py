@@ -64,6 +64,10 @@ def draw_ids(kind, n, rows, gen):
     (4096, 1023, 24, "uniform"), (5000, 1024, 40, "outside"), (12288, 45, 32, "skewed"), (12289, 45, 32, "skewed"),
     (9001, 50257, 77, "skewed"), (20000, 2000, 771, "uniform"), (40000, 5, 64, "same"), (40000, 300, 96, "reversed"),
     (30000, 131072, 256, "skewed"), (300000, 1000, 8, "skewed"), (270000, 2097153, 2, "outside"),
+    # few positions (128 at most, one launch): every one the same, none twice, some outside; wide rows, a row of several
+    # segments, a large table; one position more
+    (128, 45, 32, "same"), (128, 300, 33, "reversed"), (128, 1000, 700, "skewed"), (127, 9, 1, "uniform"),
+    (100, 131072, 8, "outside"), (3, 5000, 5000, "uniform"), (64, 33000, 2051, "skewed"), (129, 300, 33, "skewed"),
     # a table of few rows (64 at most): its last size, one more row, one more position than its blocks take, wide rows
     (255, 64, 5, "uniform"), (5000, 64, 130, "outside"), (5000, 65, 130, "outside"), (65536, 45, 33, "skewed"),
     (65537, 45, 33, "skewed"), (4097, 10, 4096, "reversed"), (4097, 10, 4097, "reversed"), (4095, 63, 8, "sorted"),
@@ -82,7 +86,7 @@ def test_lookup_and_gradient(dev, gen, n, rows, dim, kind, dtype):
     assert torch.equal(got, hip_ops.embedding_backward(ids.int(), dout, rows, 0.6))
 
 
-@pytest.mark.parametrize("n", [1000, 20000])
+@pytest.mark.parametrize("n", [100, 1000, 20000])
 def test_padding_hides_what_its_positions_hold(dev, gen, n):
     """NaN and infinities in the gradient of padded and outside positions reach nothing; all padding gives zeros."""
     from multimodalstudio_amd import hip_ops
@@ -103,7 +107,7 @@ def test_padding_hides_what_its_positions_hold(dev, gen, n):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-@pytest.mark.parametrize("n,rows,dim", [(500, 40, 32), (30000, 300, 5), (20000, 9, 64)])
+@pytest.mark.parametrize("n,rows,dim", [(500, 40, 32), (30000, 300, 5), (20000, 9, 64), (100, 90, 37)])
 def test_accumulate_and_layouts(dev, gen, dtype, n, rows, dim):
     """Added into rows of a wider, misaligned buffer; a gradient that is a slice of a wider one; indices that are a
     column of coordinates, in more dimensions than one.  What lies beside the rows stays."""
@@ -173,7 +177,7 @@ def test_function_gradient(dev, gen):
     assert (table.grad[3] == 0).all()
 
 
-@pytest.mark.parametrize("n", [3000, 30000])
+@pytest.mark.parametrize("n", [100, 3000, 30000])
 def test_in_a_graph(dev, gen, n):
     """Lookup and gradient captured once, replayed on new indices between eager calls: the eager results' bits."""
     from multimodalstudio_amd import hip_ops
