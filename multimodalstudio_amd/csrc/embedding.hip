@@ -8,6 +8,11 @@
 // that lie inside a run are finished there; the pieces of a row that crosses runs go to the workspace and a second
 // launch adds them in order.  Rows that do not occur are found by a search in the sorted list and written as zeros by
 // further blocks of the same launch, but for the first rows, which the sort's launches clear beside their few blocks.
+// Tables of at most 64 rows and calls of at most 128 positions take two launches and one.
+//
+// Lookup of 16384 x 4096 bf16: 32 us, 5.6 TB/s of rows written and different rows read (a copy reaches 5.1, a fill 6.8).
+// Gradient of 65536 x 2048 bf16 into 131072 rows: 178 us, 4.5 TB/s of both; the sort's share of it hides behind the
+// clearing of the first rows.
 #include "common.h"
 
 #include <algorithm>
@@ -500,7 +505,8 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(Grad G, T* __restri
 
 // ---- a table of few rows ------------------------------------------------------------------------------------------
 // Blocks sort and sum 256 positions each and leave a sum per row that occurs among them; a second launch adds those
-// up, block after block.  (Per-view codes: 10240 positions, 45 rows, 32 values.)
+// up, block after block.  (Per-view codes, 10240 positions of 45 rows of 32 fp32 values: 12 us a call, 24 by the sort;
+// the GPU is through with them in 9.)
 constexpr int kFewRows = 64, kFewTile = 256, kFewBits = 7;   // keys 0 .. 64
 
 struct Few {

@@ -5,11 +5,16 @@
 //   X <- a X + (b A + c A A) X,  A = X X^T                                      `steps` times
 //   p <- decay p - lr scale X
 //
-// Three products a step, all "rows times rows" (k contiguous in both operands): A = X X^T reads the rows of X; A A the
-// rows of A, which is symmetric; the last one the rows of B = b A + c A A and of X^T, so every product's epilogue
-// writes the operand layouts that the next ones read (X and X^T, or both triangles) and the loop needs no transposing
-// load.  A and B are symmetric: only tiles on or below the diagonal are computed, the others are written as mirrors --
-// 3 r^2 c + r^3 multiply-adds a step in place of 4 r^2 c + 2 r^3.
+// Three products a step: A = X X^T from the rows of X; A A from the rows of A, which is symmetric; B X, B = b A + c A A,
+// from the rows of B and, by transposing LDS loads, the rows of X.  So X is kept in one order only.  A and B are
+// symmetric: only tiles on or below the diagonal are computed, the others are written as mirrors -- 3 r^2 c + r^3
+// floating-point operations a step in place of 4 r^2 c + 2 r^3.
+//
+// What bounds it.  Large matrices: the products, at the rate the card's power allows (4096 x 4096, prec 1: 1.41 ms, 975
+// TFLOP/s of the operations above; a library product of that size reaches 1040); prec 0 does three products for one
+// (2048-wide block of six matrices: 4.33 ms, 1030 TFLOP/s of its fp16 products).  Stacks of 1024 x 4096: the iterates' way
+// through memory beside them (8 bytes an element and step, with the operand 10).  Small ones: 2 + 3 steps launches of 4 to
+// 8 us, each no more than one block's loads, products and stores in a row (the renderer's 19 matrices: 129 us).
 //
 // Precision.  Operands are fp16 with |X| <= 1.2 held as 2^10 X (entries from 2^-24 of the largest possible keep their
 // bits); fp32 accumulators.
@@ -18,12 +23,13 @@
 //           which the map's slope (up to a^5 = 485 for small singular values) takes to 3e-5 .. 2e-4.
 //   prec 1  one fp16 product.  X itself keeps hi + lo and a X is added from those in fp32: rounding only enters
 //           through (b A + c A A) X, so the result is 0.9e-3 .. 1.4e-3 off, under bf16's own 1.7e-3 (X rounded to fp16
-//           between steps: up to 1.2e-2 where a few directions are far stronger than the rest).  Small matrices
-//           (64-wide tiles) run prec 0 all the same: they wait for launches and loads, not for products, and with few
+//           between steps: up to 1.2e-2 where a few directions are far stronger than the rest).  Matrices of up to 128
+//           rows or columns run prec 0 all the same: they wait for launches and loads, not for products, and with few
 //           entries to average over, single products are up to 3.8e-3 off.
 //
 // Every matrix of a call takes part in the same 2 + 3 steps launches; a block finds its matrix and tile by blockIdx.
-// Padded rows and columns (to the tile) are zeros in every operand, so the product loop has no bounds checks.
+// Operands are padded to 64 rows and columns, with zeros, and what a wider tile has past them is never stored, so the
+// product loop has no bounds checks.
 #include "common.h"
 #include "chain_common.h"
 
@@ -893,9 +899,9 @@ void launch_product(int tile, NsTable* T, int64_t blocks, const NsStep& S, float
 #define NS_LAUNCH(TILE, WM, WN, NBUF)                                                                            \
   hipLaunchKernelGGL((ns_product_kernel<TILE, WM, WN, NBUF, W, PHASE>), grid, dim3((TILE / WM) * (TILE / WN) * 64), 0, \
                      s, T, S, a, b, c, parity, bf16, chunk, partial)
-  // 16 waves a CU where registers and LDS allow it: 8-wave blocks of 128 two at a time (482 us against 494 with 4 waves,
-  // X of muon's four 2048 x 2048 and two 2048 x 5632 in prec 0), 16 of 64 x 64 rather than 8 of 128 x 64 for 256 (483,
-  // 509), 4-wave blocks of 64 three at a time
+  // 16 waves a CU where registers and LDS allow it: 8-wave blocks of 128 two at a time (X of four 2048 x 2048 and two
+  // 2048 x 5632 in prec 0: 2% faster than 4 waves), 16 of 64 x 64 rather than 8 of 128 x 64 for 256 (5%), 4-wave blocks
+  // of 64 three at a time
   if (tile == 64) NS_LAUNCH(64, 32, 32, 3);
   else if (tile == 128) NS_LAUNCH(128, 64, 32, 2);
   else if (tile == 192) NS_LAUNCH(192, 64, 48, 3);
