@@ -432,7 +432,7 @@ def _rows2d(t: torch.Tensor, dim: int) -> torch.Tensor:
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """out[..., :] = scale * table[ids[...], :]; ids int32 / int64 of any shape, table [rows, dim] float32, bfloat16 or
-    float16.  An index outside the table gives a row of zeros."""
+    float16.  An index outside the table gives a row of zeros.  Without autograd history (EmbeddingFunction has it)."""
     dt = _check_table(ids, table, "the table")
     if table.dim() != 2 or table.shape[0] == 0 or table.shape[1] == 0:
         raise ValueError(f"embedding: the table must be [rows, dim], got {tuple(table.shape)}")
@@ -491,7 +491,8 @@ def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: 
 
 
 class EmbeddingFunction(torch.autograd.Function):
-    """Learned row table forward / backward on the HIP kernels: apply(ids, table, scale=1.0, padding_idx=None)."""
+    """Learned row table forward / backward on the HIP kernels: apply(ids, table, scale=1.0, padding_idx=None).  Once
+    differentiable: a derivative of its gradient raises."""
 
     @staticmethod
     def forward(ctx, ids, table, scale: float = 1.0, padding_idx: Optional[int] = None):
@@ -500,6 +501,7 @@ class EmbeddingFunction(torch.autograd.Function):
         return embedding(ids, table, scale)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
         rows, scale, padding_idx = ctx.cfg

@@ -177,6 +177,17 @@ def test_function_gradient(dev, gen):
     assert (table.grad[3] == 0).all()
 
 
+def test_second_derivative_is_refused(dev, gen):
+    """The gradient's own gradient would be lost without a word: it raises."""
+    from multimodalstudio_amd.hip_ops import EmbeddingFunction
+    table = torch.randn(9, 12, device="cuda", generator=gen, requires_grad=True)
+    ids = torch.randint(0, 9, (50,), device="cuda", generator=gen)
+    out = EmbeddingFunction.apply(ids, table)
+    (first,) = torch.autograd.grad(out.square().sum(), table, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        first.sum().backward()
+
+
 @pytest.mark.parametrize("n", [100, 3000, 30000])
 def test_in_a_graph(dev, gen, n):
     """Lookup and gradient captured once, replayed on new indices between eager calls: the eager results' bits."""
