@@ -34,6 +34,7 @@
 #include "chain_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -505,10 +506,10 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
 #pragma unroll
     for (int j = 0; j < (APART ? FN : 1); ++j) cross[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
   // lo lo too where few singular values leave little to average (3 x 64: 1.1 of float32 products' error on average, 1.6
-  // without; from 64 rows it would be 0.5 .. 0.7 for 0.5 .. 0.8, and 7% slower)
-  const bool narrow = APART && L.rp == 64;
+  // without; from 64 rows it would be 0.5 .. 0.7 for 0.5 .. 0.8, and 7% slower).  Tiles that cannot keep them apart go
+  // over such a matrix twice: first everything but hi hi, then hi hi (beside larger matrices, 3 x 64: 1.2, 1.9 without).
+  const bool narrow = W == 2 && L.rp == 64;
   const int frow = lane & 15;
-  for (int s = 0; s < NBUF - 1 && s < stages; ++s) issue(s);
   const int fchunk = ((lane >> 4) ^ (lane & 7)) << 4;
   // the lane's place in the two halves of 32 columns of X's rows, and the distance from hi to lo or to the next 32 rows
   int ftr[FN], fnext;
@@ -531,50 +532,66 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
     }
     return v;
   };
-  for (int s = 0; s < stages; ++s) {
-    // stage s has arrived once only the loads issued after it are outstanding; all waves are then past stage s - 1
-    if (s + NBUF - 2 < stages) wait_vm_barrier<(NBUF - 2) * LOADS>();
-    else wait_vm_barrier<0>();
-    if (s + NBUF - 1 < stages) issue(s + NBUF - 1);
-    const char* pa = lds + (s % NBUF) * STAGE + (wm * WM + frow) * 128;
-    const char* pq = lds + (s % NBUF) * STAGE + (TILE + (PHASE >= PHASE_X ? 0 : wn * WN + frow)) * 128;
-    half8 a0[FM], a1[FM], b0[FN], b1[FN];
+  enum { ALL, SMALL, LARGE };   // which products
+  const auto sweep = [&](auto which) {
+    constexpr int MODE = decltype(which)::value;
+    for (int s = 0; s < NBUF - 1 && s < stages; ++s) issue(s);
+    for (int s = 0; s < stages; ++s) {
+      // stage s has arrived once only the loads issued after it are outstanding; all waves are then past stage s - 1
+      if (s + NBUF - 2 < stages) wait_vm_barrier<(NBUF - 2) * LOADS>();
+      else wait_vm_barrier<0>();
+      if (s + NBUF - 1 < stages) issue(s + NBUF - 1);
+      const char* pa = lds + (s % NBUF) * STAGE + (wm * WM + frow) * 128;
+      const char* pq = lds + (s % NBUF) * STAGE + (TILE + (PHASE >= PHASE_X ? 0 : wn * WN + frow)) * 128;
+      half8 a0[FM], a1[FM], b0[FN], b1[FN];
 #pragma unroll
-    for (int i = 0; i < FM; ++i) a0[i] = *(const half8*)(pa + i * 2048 + fchunk);
-#pragma unroll
-    for (int j = 0; j < FN; ++j)
-      b0[j] = PHASE >= PHASE_X ? column(pq + ftr[j]) : *(const half8*)(pq + j * 2048 + fchunk);
-#pragma unroll
-    for (int j = 0; j < FN; ++j)
-      b1[j] = PHASE >= PHASE_X ? column(pq + ftr[j] + fnext) : *(const half8*)(pq + j * 2048 + (fchunk ^ 64));
-#pragma unroll
-    for (int i = 0; i < FM; ++i) a1[i] = *(const half8*)(pa + i * 2048 + (fchunk ^ 64));
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
+      for (int i = 0; i < FM; ++i) a0[i] = *(const half8*)(pa + i * 2048 + fchunk);
 #pragma unroll
       for (int j = 0; j < FN; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0[i], b0[j], acc[i][j], 0, 0, 0);
+        b0[j] = PHASE >= PHASE_X ? column(pq + ftr[j]) : *(const half8*)(pq + j * 2048 + fchunk);
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+      for (int j = 0; j < FN; ++j)
+        b1[j] = PHASE >= PHASE_X ? column(pq + ftr[j] + fnext) : *(const half8*)(pq + j * 2048 + (fchunk ^ 64));
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        floatx4& to = APART ? cross[APART ? i : 0][APART ? j : 0] : acc[i][j];
-        if (W == 2) to = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0[i], b1[j], to, 0, 0, 0);
+      for (int i = 0; i < FM; ++i) a1[i] = *(const half8*)(pa + i * 2048 + (fchunk ^ 64));
+      if (MODE != SMALL)
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0[i], b0[j], acc[i][j], 0, 0, 0);
+      if (MODE == LARGE) continue;
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          floatx4& to = APART ? cross[APART ? i : 0][APART ? j : 0] : acc[i][j];
+          if (W == 2) to = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0[i], b1[j], to, 0, 0, 0);
+        }
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          floatx4& to = APART ? cross[APART ? i : 0][APART ? j : 0] : acc[i][j];
+          to = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1[i], W == 2 ? b0[j] : b1[j], to, 0, 0, 0);
+        }
+      if (MODE == SMALL || (APART && narrow)) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) {
+            floatx4& to = APART ? cross[APART ? i : 0][APART ? j : 0] : acc[i][j];
+            to = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1[i], b1[j], to, 0, 0, 0);
+          }
       }
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        floatx4& to = APART ? cross[APART ? i : 0][APART ? j : 0] : acc[i][j];
-        to = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1[i], W == 2 ? b0[j] : b1[j], to, 0, 0, 0);
-      }
-    if (APART && narrow) {
-#pragma unroll
-      for (int i = 0; i < (APART ? FM : 1); ++i)
-#pragma unroll
-        for (int j = 0; j < (APART ? FN : 1); ++j)
-          cross[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1[i], b1[j], cross[i][j], 0, 0, 0);
     }
+  };
+  if (W == 2 && !APART && narrow) {
+    sweep(std::integral_constant<int, SMALL>{});
+    __syncthreads();
+    sweep(std::integral_constant<int, LARGE>{});
+  } else {
+    sweep(std::integral_constant<int, ALL>{});
   }
   if (APART) {
 #pragma unroll
