@@ -188,6 +188,23 @@ def test_second_derivative_is_refused(dev, gen):
         first.sum().backward()
 
 
+def test_two_calls_at_once(dev, gen):
+    """Gradients on two streams that run together: each gives its own bits."""
+    from multimodalstudio_amd import hip_ops
+    calls = [(torch.randint(0, rows, (n,), device="cuda", generator=gen), torch.randn(n, 96, device="cuda", generator=gen), rows)
+             for n, rows in ((100, 5000), (20000, 3000), (9000, 45), (40000, 70000))]
+    want = [hip_ops.embedding_backward(*c) for c in calls]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for k, c in enumerate(calls):
+            with torch.cuda.stream(streams[k % 2]):
+                got.append(hip_ops.embedding_backward(*c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
 @pytest.mark.parametrize("n", [100, 3000, 30000])
 def test_in_a_graph(dev, gen, n):
     """Lookup and gradient captured once, replayed on new indices between eager calls: the eager results' bits."""

@@ -298,6 +298,23 @@ def test_another_stream(dev, gen):
         assert torch.equal(o, want)
 
 
+def test_two_calls_at_once(dev, gen):
+    """Calls on two streams that run together, their sums over long rows split: each gives its own bits."""
+    from multimodalstudio_amd import hip_ops
+    calls = [[gradient((40, 5000), gen, torch.float32), gradient((300, 4096), gen, torch.float32)],
+             [gradient((700, 8192), gen, torch.bfloat16), gradient((9, 3000), gen, torch.bfloat16)]]
+    want = [hip_ops.newton_schulz(c) for c in calls]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, c in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append(hip_ops.newton_schulz(c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for g, w in zip(got, want) for x, y in zip(g, w))
+
+
 def test_refusals(dev):
     from multimodalstudio_amd import hip_ops
     p, m = torch.zeros(6, 8, device="cuda"), torch.zeros(6, 8, device="cuda")
