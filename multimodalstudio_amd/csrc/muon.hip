@@ -474,21 +474,24 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
     for (int j = 0; j < FN; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   // what the epilogue adds to the product: with 64-wide tiles, whose time is waiting, brought along with the operands
-  constexpr int OWN = TILE == 64 && PHASE != PHASE_A ? 64 * TILE / 4 / NT : 0;
-  half4 own_hi[OWN + 1], own_lo[OWN + 1];
-  // (the last product's results go to rows of the caller's: threads along the row; others as the operands lie: 8 threads
+  constexpr int G = PHASE == PHASE_LAST ? 4 : 8;   // columns of a thread (8: 1% of all but the large prec 1 products)
+  typedef _Float16 halfg __attribute__((ext_vector_type(G)));
+  typedef MMS_GLOBAL halfg ghalfg;
+  constexpr int OWN = TILE == 64 && PHASE != PHASE_A ? 64 * TILE / G / NT : 0;
+  halfg own_hi[OWN + 1], own_lo[OWN + 1];
+  // (the last product's results go to rows of the caller's: threads along the row; others as the operands lie: 4 threads
   // for 32 columns, then the next row)
   const auto place = [](int e, int& i, int& j) {
     if (PHASE == PHASE_LAST) { i = e / (TILE / 4); j = e % (TILE / 4) * 4; }
-    else { i = (e >> 3) & 63; j = (e >> 9) * 32 + (e & 7) * 4; }
+    else { i = e / (32 / G) & 63; j = e / (64 * 32 / G) * 32 + e % (32 / G) * G; }
   };
-  const auto own = [&](int i, int j, half4& hi, half4& lo) {
+  const auto own = [&](int i, int j, halfg& hi, halfg& lo) {
     const int64_t d = at<W>(ti * TILE + i, L.rp, tj * TILE + j);
     const ghalf* x = PHASE == PHASE_B ? P : (const ghalf*)(ws + L.x(parity));
-    hi = *(const ghalf4*)(x + d);
-    if (W == 2) lo = *(const ghalf4*)(x + d + 32);
-    else if (PHASE >= PHASE_X) lo = *(const ghalf4*)((const ghalf*)(ws + L.xlo()) + d);
-    else lo = half4{0, 0, 0, 0};
+    hi = *(const ghalfg*)(x + d);
+    if (W == 2) lo = *(const ghalfg*)(x + d + 32);
+    else if (PHASE >= PHASE_X) lo = *(const ghalfg*)((const ghalf*)(ws + L.xlo()) + d);
+    else lo = halfg(0);
   };
 #pragma unroll
   for (int o = 0; o < OWN; ++o) {
@@ -708,36 +711,36 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
     __syncthreads();
     const int i0 = ti * TILE + s * 64, j0 = tj * TILE;
 #pragma unroll
-    for (int o = 0; o < 64 * TILE / 4 / NT; ++o) {
+    for (int o = 0; o < 64 * TILE / G / NT; ++o) {
       int i, j;
       place(threadIdx.x + o * NT, i, j);
       if (TILE > 64 && j0 + j >= width) continue;
-      float v[4];
+      float v[G];
 #pragma unroll
-      for (int z = 0; z < 4; ++z) v[z] = slab[i * LD + j + z];
-      half4 hi, lo;
+      for (int z = 0; z < G; ++z) v[z] = slab[i * LD + j + z];
+      halfg hi, lo;
       if (PHASE != PHASE_A) {
         if (OWN) { hi = own_hi[OWN ? o : 0]; lo = own_lo[OWN ? o : 0]; }
         else own(s * 64 + i, j, hi, lo);
 #pragma unroll
-        for (int z = 0; z < 4; ++z) {
+        for (int z = 0; z < G; ++z) {
           const float y = (float)hi[z] + (float)lo[z];
           v[z] = PHASE == PHASE_B ? __builtin_fmaf(cb, y, cc * v[z]) : __builtin_fmaf(ca, y, v[z]);
         }
       }
       if (PHASE == PHASE_B || PHASE == PHASE_LAST) {
 #pragma unroll
-        for (int z = 0; z < 4; ++z) slab[i * LD + j + z] = v[z];
+        for (int z = 0; z < G; ++z) slab[i * LD + j + z] = v[z];
       }
       if (PHASE == PHASE_LAST) {
         if (!tall) put(i0 + i, j0 + j, v);
       } else {
-        split_n<4>(v, (_Float16*)&hi, (_Float16*)&lo);
+        split_n<G>(v, (_Float16*)&hi, (_Float16*)&lo);
         const int64_t d = at<W>(i0 + i, L.rp, j0 + j);
         ghalf* to = PHASE == PHASE_X ? X : D;
-        *(ghalf4*)(to + d) = hi;
-        if (W == 2) *(ghalf4*)(to + d + 32) = lo;
-        else if (PHASE == PHASE_X) *(ghalf4*)(Xlo + d) = lo;
+        *(ghalfg*)(to + d) = hi;
+        if (W == 2) *(ghalfg*)(to + d + 32) = lo;
+        else if (PHASE == PHASE_X) *(ghalfg*)(Xlo + d) = lo;
       }
     }
     // the other order: the mirrored triangle, or a tall result
