@@ -10,11 +10,11 @@
 // symmetric: only tiles on or below the diagonal are computed, the others are written as mirrors -- 3 r^2 c + r^3
 // floating-point operations a step in place of 4 r^2 c + 2 r^3.
 //
-// What bounds it.  Large matrices: the products, at the rate the card's power allows (4096 x 4096, prec 1: 1.41 ms, 975
-// TFLOP/s of the operations above; a library product of that size reaches 1040); prec 0 does three products for one
-// (2048-wide block of six matrices: 4.33 ms, 1030 TFLOP/s of its fp16 products).  Stacks of 1024 x 4096: the iterates' way
-// through memory beside them (8 bytes an element and step, with the operand 10).  Small ones: 2 + 3 steps launches of 4 to
-// 8 us, each no more than one block's loads, products and stores in a row (the renderer's 19 matrices: 129 us).
+// What bounds it.  Large matrices: the products, at the rate the card's power allows (4096 x 4096, prec 1: 1.39 .. 1.46
+// ms, 940 .. 990 TFLOP/s of the operations above; a library product of that size reaches 1040); prec 0 does three products
+// for one (a 2048-wide block of six matrices: 4.27 .. 4.54 ms, 980 .. 1040 TFLOP/s of its fp16 products).  Stacks of 1024 x
+// 4096: the iterates' way through memory beside them (8 bytes an element and step, with the operand 10).  Small ones: 2 +
+// 3 steps launches of 4 to 8 us, each one block's loads, products and stores in a row (the renderer's 19 matrices: 130 us).
 //
 // Precision.  Operands are fp16 with |X| <= 1.2 held as 2^10 X (entries from 2^-24 of the largest possible keep their
 // bits); fp32 accumulators.
