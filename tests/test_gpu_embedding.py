@@ -188,6 +188,24 @@ def test_second_derivative_is_refused(dev, gen):
         first.sum().backward()
 
 
+@pytest.mark.parametrize("n", [100, 5000])
+def test_offsets_past_32_bits(dev, gen, n):
+    """A table of more than 2^31 values: rows on both sides of that, and what lies between them is zeros."""
+    from multimodalstudio_amd import hip_ops
+    dim = 1030
+    rows = 2 ** 31 // dim + 4000
+    ids = torch.cat([torch.randint(0, 50, (n // 2,), device="cuda", generator=gen),
+                     rows - 1 - torch.randint(0, 50, (n - n // 2,), device="cuda", generator=gen)])
+    dout = torch.randn(n, dim, device="cuda", generator=gen).to(torch.bfloat16)
+    grad = hip_ops.embedding_backward(ids, dout, rows, 0.5)
+    ends = torch.cat([grad[:50], grad[-50:]])
+    check(ends, torch.where(ids < 50, ids, ids - (rows - 100)), dout, 100, 0.5)
+    assert not any(grad[r:r + 100000].any() for r in range(50, rows - 50, 100000)
+                   if r + 100000 <= rows - 50) and not grad[rows - 100050:rows - 50].any()
+    out = hip_ops.embedding(ids, grad, 2.0)
+    assert torch.equal(out, (grad[ids].float() * 2.0).to(torch.bfloat16))
+
+
 def test_two_calls_at_once(dev, gen):
     """Gradients on two streams that run together: each gives its own bits."""
     from multimodalstudio_amd import hip_ops

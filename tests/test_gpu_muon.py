@@ -298,6 +298,19 @@ def test_another_stream(dev, gen):
         assert torch.equal(o, want)
 
 
+def test_offsets_past_32_bits(dev, gen):
+    """A stack of more than 2^31 elements: its first, middle and last matrix."""
+    from multimodalstudio_amd import hip_ops
+    few = gradient((3, 1024, 1100), gen, torch.bfloat16)
+    n = 2 ** 31 // (1024 * 1100) + 2
+    stack = few[1].expand(n, -1, -1).contiguous()
+    stack[0], stack[n - 1] = few[0], few[2]
+    out = hip_ops.newton_schulz(stack)
+    for k, g in ((0, few[0]), (n // 2, few[1]), (n - 1, few[2])):
+        want = iterate(g, torch.float64)
+        assert rel(out[k], want) <= tolerance(g, want), k
+
+
 def test_two_calls_at_once(dev, gen):
     """Calls on two streams that run together, their sums over long rows split: each gives its own bits."""
     from multimodalstudio_amd import hip_ops
