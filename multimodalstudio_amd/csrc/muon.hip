@@ -16,11 +16,15 @@
 // 4096: the iterates' way through memory beside them (8 bytes an element and step, with the operand 10).  Small ones: 2 +
 // 3 steps launches of 4 to 8 us, each one block's loads, products and stores in a row (the renderer's 19 matrices: 130 us).
 //
-// Precision.  Operands are fp16 with |X| <= 1.2 held as 2^10 X (entries from 2^-24 of the largest possible keep their
-// bits); fp32 accumulators.
-//   prec 0  x = hi + lo, both fp16 (22 bits); a product is hi hi + hi lo + lo hi: as near the definition as fp32
-//           products, at a third of the fp16 matrix rate (fp32 MFMA: a sixteenth).  bf16 pairs hold 16 bits only,
-//           which the map's slope (up to a^5 = 485 for small singular values) takes to 3e-5 .. 2e-4.
+// Precision.  Operands are fp16, X, A and B each times the largest power of two that its entries allow: they are bounded
+// by singular values, those by the coefficients (2^15 X, 2^15 A, 2^14 B for a, b, c = 3.4445, -4.7750, 2.0315); fp32
+// accumulators.
+//   prec 0  x = hi + 2^-6 lo, both fp16; a product is hi hi + 2^-6 (hi lo + lo hi): as near the definition as fp32
+//           products, at a third of the fp16 matrix rate (fp32 MFMA: a sixteenth).  Entries of X from 2^-23 on -- a
+//           gradient's from 2^-23 of its norm -- keep 22 bits, smaller ones are within 2^-46.  So the small part of an
+//           uneven gradient keeps its accuracy too: noise beside an entry of 10^6 is 1.2e-7 off (with lo itself in fp16
+//           and a unit of 2^10 for all: 1.8e-5; float32 products 0.8e-7).  bf16 pairs hold 16 bits only, which the
+//           map's slope (up to a^5 = 485 for small singular values) takes to 3e-5 .. 2e-4.
 //   prec 1  one fp16 product.  X itself keeps hi + lo and a X is added from those in fp32: rounding only enters
 //           through (b A + c A A) X, so the result is 0.9e-3 .. 1.4e-3 off, under bf16's own 1.7e-3 (X rounded to fp16
 //           between steps: up to 1.2e-2 where a few directions are far stronger than the rest).  Matrices of up to 128
@@ -52,8 +56,9 @@ typedef __attribute__((address_space(3))) short4v lds_short4;
 
 constexpr int kMaxMatrices = 4096;       // (or stacks) per call
 constexpr int kNsItems = 48;             // matrices (or stacks of them) per launch: the argument struct stays < 4 KB
-constexpr float kScale = 1024.f;         // fp16 operands hold 2^10 times their value
-constexpr float kDescale = 1.f / 1024.f; // a product of two of them, back to 2^10 times its value
+constexpr float kLow = 64.f;             // what hi leaves of a value is held 2^6 times
+constexpr float kUnlow = 1.f / 64.f;
+constexpr float kHalfMax = 60000.f;      // fp16's largest value, less a margin for roundings
 constexpr int kNormBlocks = 1024;        // blocks per matrix that sum squares, at most
 constexpr int kNormElems = 8192;         // elements per such block, at least
 constexpr int64_t kMaxBlocks = 1 << 23;  // of a launch (times its threads: below 2^32)
@@ -99,6 +104,7 @@ struct NsStep {
   const float* hyper;       // device [decay, -lr], or null: the two values
   float decay, neg_lr;
   double eps;
+  float unit[3];            // fp16 operands hold X, A and B = b A + c A A times these powers of two
 };
 
 // The workspace of one matrix: norm partials, then the fp16 operands.  W: 2 with hi and lo (32 of each in turn along
@@ -262,7 +268,7 @@ __device__ __forceinline__ void split_n(const float* v, _Float16* hi, _Float16* 
 #pragma unroll
   for (int q = 0; q < N; ++q) {
     hi[q] = (_Float16)v[q];
-    lo[q] = (_Float16)(v[q] - (float)hi[q]);
+    lo[q] = (_Float16)((v[q] - (float)hi[q]) * kLow);
   }
 }
 
@@ -331,7 +337,7 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const NsTable* __restrict_
   __syncthreads();
   double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
   norm = norm < S.eps ? S.eps : norm;
-  const double inv = (double)kScale / norm;
+  const double inv = (double)S.unit[0] / norm;
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     const float gi = gv[e] * clip;
@@ -382,7 +388,7 @@ __device__ __forceinline__ const char* uniform(const char* p) {
 // bytes): the 8 rows that 32 lanes read are in different banks.  So X^T is kept nowhere.
 template <int TILE, int WM, int WN, int NBUF, int W, int PHASE>
 __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_kernel(
-    NsTable* __restrict__ T, NsStep S, float ca, float cb, float cc, int parity, int bf16, int chunk,
+    NsTable* __restrict__ T, NsStep S, float mul, float ca, float cb, float cc, int parity, int bf16, int chunk,
     uint64_t* __restrict__ partial) {
   constexpr int NWM = TILE / WM, NWN = TILE / WN, NW = NWM * NWN, NT = NW * 64;
   constexpr int STAGE = 2 * TILE * 128;          // bytes
@@ -500,17 +506,24 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
     own(i, j, own_hi[o], own_lo[o]);
   }
 
-  // hi lo + lo hi on their own where registers allow it: a matrix instruction rounds its sum each time, and these are
-  // 2^-11 of hi hi (the renderer's matrices: 0.5 of float32 products' error, 0.7 in one sum)
-  constexpr bool APART = W == 2 && TILE == 64;
-  floatx4 cross[APART ? FM : 1][APART ? FN : 1];
+  // lo is 2^6 times what it stands for, so that it keeps its bits where hi is small; hi lo + lo hi then count 2^-6.  They
+  // have a sum of their own, up to tiles of 192: a matrix instruction rounds its sum each time, and these are 2^-11 of
+  // hi hi (the renderer's matrices: 0.5 of float32 products' error, 0.7 in one sum).  256-wide tiles have no registers for
+  // two sums: there hi, once multiplied by hi, is itself taken 2^-6 times.
+  constexpr bool APART = W == 2 && TILE < 256;
+  constexpr bool LEAST = W == 2 && TILE == 64;   // a third sum, of lo lo
+  floatx4 cross[APART ? FM : 1][APART ? FN : 1], least[LEAST ? FM : 1][LEAST ? FN : 1];
 #pragma unroll
   for (int i = 0; i < (APART ? FM : 1); ++i)
 #pragma unroll
     for (int j = 0; j < (APART ? FN : 1); ++j) cross[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < (LEAST ? FM : 1); ++i)
+#pragma unroll
+    for (int j = 0; j < (LEAST ? FN : 1); ++j) least[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
   // lo lo too where few singular values leave little to average (3 x 64: 1.1 of float32 products' error on average, 1.6
-  // without; from 64 rows it would be 0.5 .. 0.7 for 0.5 .. 0.8, and 7% slower).  Tiles that cannot keep them apart go
-  // over such a matrix twice: first everything but hi hi, then hi hi (beside larger matrices, 3 x 64: 1.2, 1.9 without).
+  // without; from 64 rows it would be 0.5 .. 0.7 for 0.5 .. 0.8, and 7% slower).  Tiles that lack a sum for it go over such
+  // a matrix once more for each unit.
   const bool narrow = W == 2 && L.rp == 64;
   const int frow = lane & 15;
   const int fchunk = ((lane >> 4) ^ (lane & 7)) << 4;
@@ -535,8 +548,14 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
     }
     return v;
   };
-  enum { ALL, SMALL, LARGE };   // which products
-  const auto sweep = [&](auto which) {
+  const auto multiply = [&](const half8 (&a)[FM], const half8 (&b)[FN], auto& to) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) to[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], b[j], to[i][j], 0, 0, 0);
+  };
+  enum { ALL, LOW_LOW, CROSS, LARGE };   // which products
+  const auto sweep = [&](auto which, auto& to, auto& small) {
     constexpr int MODE = decltype(which)::value;
     for (int s = 0; s < NBUF - 1 && s < stages; ++s) issue(s);
     for (int s = 0; s < stages; ++s) {
@@ -557,50 +576,53 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
         b1[j] = PHASE >= PHASE_X ? column(pq + ftr[j] + fnext) : *(const half8*)(pq + j * 2048 + (fchunk ^ 64));
 #pragma unroll
       for (int i = 0; i < FM; ++i) a1[i] = *(const half8*)(pa + i * 2048 + (fchunk ^ 64));
-      if (MODE != SMALL)
+      if (MODE == ALL || MODE == LARGE) multiply(a0, b0, to);
+      if (W == 1) multiply(a1, b1, to);
+      if (W == 2 && !APART && MODE == ALL) {
 #pragma unroll
-        for (int i = 0; i < FM; ++i)
+        for (int i = 0; i < FM; ++i) a0[i] *= (_Float16)kUnlow;
 #pragma unroll
-          for (int j = 0; j < FN; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0[i], b0[j], acc[i][j], 0, 0, 0);
-      if (MODE == LARGE) continue;
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          floatx4& to = APART ? cross[APART ? i : 0][APART ? j : 0] : acc[i][j];
-          if (W == 2) to = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0[i], b1[j], to, 0, 0, 0);
-        }
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          floatx4& to = APART ? cross[APART ? i : 0][APART ? j : 0] : acc[i][j];
-          to = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1[i], W == 2 ? b0[j] : b1[j], to, 0, 0, 0);
-        }
-      if (MODE == SMALL || (APART && narrow)) {
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-          for (int j = 0; j < FN; ++j) {
-            floatx4& to = APART ? cross[APART ? i : 0][APART ? j : 0] : acc[i][j];
-            to = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1[i], b1[j], to, 0, 0, 0);
-          }
+        for (int j = 0; j < FN; ++j) b0[j] *= (_Float16)kUnlow;
       }
+      if (W == 2 && (MODE == ALL || MODE == CROSS)) {
+        multiply(a0, b1, small);
+        multiply(a1, b0, small);
+      }
+      if (MODE == LOW_LOW) multiply(a1, b1, small);
+      if constexpr (LEAST)
+        if (narrow) multiply(a1, b1, least);
     }
   };
-  if (W == 2 && !APART && narrow) {
-    sweep(std::integral_constant<int, SMALL>{});
-    __syncthreads();
-    sweep(std::integral_constant<int, LARGE>{});
-  } else {
-    sweep(std::integral_constant<int, ALL>{});
-  }
-  if (APART) {
+  const auto lower = [&](auto& x) {
+#pragma unroll
+    for (auto& row : x)
+#pragma unroll
+      for (floatx4& v : row) v *= kUnlow;
+  };
+  if constexpr (APART) {
+    if (!LEAST && narrow) {
+      sweep(std::integral_constant<int, LOW_LOW>{}, acc, cross);
+      lower(cross);
+      __syncthreads();
+    }
+    sweep(std::integral_constant<int, ALL>{}, acc, cross);
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i][j] += cross[APART ? i : 0][APART ? j : 0];
+      for (int j = 0; j < FN; ++j) {
+        if (LEAST) cross[i][j] += least[LEAST ? i : 0][LEAST ? j : 0] * kUnlow;
+        acc[i][j] += cross[i][j] * kUnlow;
+      }
+  } else if (W == 2 && narrow) {
+    sweep(std::integral_constant<int, LOW_LOW>{}, acc, acc);
+    lower(acc);
+    __syncthreads();
+    sweep(std::integral_constant<int, CROSS>{}, acc, acc);
+    lower(acc);
+    __syncthreads();
+    sweep(std::integral_constant<int, LARGE>{}, acc, acc);
+  } else {
+    sweep(std::integral_constant<int, ALL>{}, acc, acc);
   }
   __syncthreads();
   if (PHASE == PHASE_A && parts > 1) {
@@ -656,7 +678,7 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
   const bool tall = it.rows > it.cols;
   gchar* out = PHASE == PHASE_LAST ? (gchar*)it.p + k * it.bsp * (bf16 ? 2 : 4) : nullptr;
   const float decay = PHASE == PHASE_LAST && it.m ? (S.hyper ? S.hyper[0] : S.decay) : 0.f;
-  const float gain = PHASE == PHASE_LAST ? (it.m ? (S.hyper ? S.hyper[1] : S.neg_lr) * it.scale : 1.f) * kDescale : 0.f;
+  const float gain = PHASE == PHASE_LAST ? (it.m ? (S.hyper ? S.hyper[1] : S.neg_lr) * it.scale : 1.f) / S.unit[0] : 0.f;
   // 4 values to the caller's matrix, together where its rows are whole and aligned groups of 4
   const bool quads = PHASE == PHASE_LAST && it.cols % 4 == 0 && it.ldp % 4 == 0 && ((uint64_t)out & (bf16 ? 7 : 15)) == 0;
   const auto put = [&](int row, int col, const float* v) {
@@ -705,7 +727,7 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
         for (int j = 0; j < FN; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            slab[(row + (lane >> 4) * 4 + e) * LD + wn * WN + j * 16 + frow] = acc[i][j][e] * kDescale;
+            slab[(row + (lane >> 4) * 4 + e) * LD + wn * WN + j * 16 + frow] = acc[i][j][e] * mul;
       }
     }
     __syncthreads();
@@ -724,7 +746,7 @@ __global__ __launch_bounds__((TILE / WM) * (TILE / WN) * 64) void ns_product_ker
         else own(s * 64 + i, j, hi, lo);
 #pragma unroll
         for (int z = 0; z < G; ++z) {
-          const float y = (float)hi[z] + (float)lo[z];
+          const float y = __builtin_fmaf((float)lo[z], kUnlow, (float)hi[z]);
           v[z] = PHASE == PHASE_B ? __builtin_fmaf(cb, y, cc * v[z]) : __builtin_fmaf(ca, y, v[z]);
         }
       }
@@ -915,10 +937,15 @@ int64_t workspace_of(const int* order, int live, const int64_t* batch, const int
 template <int W, int PHASE>
 void launch_product(int tile, NsTable* T, int64_t blocks, const NsStep& S, float a, float b, float c, int parity,
                     int bf16, int chunk, uint64_t* partial, hipStream_t s) {
+  // a sum's factor, to hold A, A A in A's unit, B X in X's; then B's unit for A's
+  const float x = S.unit[0], aa = S.unit[1], bb = S.unit[2];
+  const float mul = PHASE == PHASE_A ? aa / (x * x) : 1.f / (PHASE == PHASE_B ? aa : bb);
+  b *= bb / aa;
+  c *= bb / aa;
   const dim3 grid((unsigned)blocks);
 #define NS_LAUNCH(TILE, WM, WN, NBUF)                                                                            \
   hipLaunchKernelGGL((ns_product_kernel<TILE, WM, WN, NBUF, W, PHASE>), grid, dim3((TILE / WM) * (TILE / WN) * 64), 0, \
-                     s, T, S, a, b, c, parity, bf16, chunk, partial)
+                     s, T, S, mul, a, b, c, parity, bf16, chunk, partial)
   // 16 waves a CU where registers and LDS allow it: 8-wave blocks of 128 two at a time (X of four 2048 x 2048 and two
   // 2048 x 5632 in prec 0: 2% faster than 4 waves), 16 of 64 x 64 rather than 8 of 128 x 64 for 256 (5%), 4-wave blocks
   // of 64 three at a time
@@ -942,12 +969,51 @@ void launch_group(const NsPlan& P, const NsArgs& A, NsTable* T, const NsStep& S,
   }
 }
 
+// The operands' units: the largest powers of two, up to 2^15, with which no entry can pass fp16's range.  Entries are at
+// most the largest singular value, which starts at 1 or less; p(s) = a s + b s^3 + c s^5 takes [0, m] onto [0, max |p|]
+// (and beyond zero), B has b t + c t^2 for t in [0, m^2].  False: some matrix's iterates leave the range.
+bool ns_units(int steps, double a, double b, double c, float (&unit)[3]) {
+  constexpr double margin = 1.01;   // roundings: a singular value may be a little larger than exactly computed
+  double m = margin, x = 0.0, poly = 0.0;
+  for (int i = 0; i < steps; ++i) {
+    x = std::max(x, m);
+    const double t = m * m;
+    double next = 0.0;
+    const auto see_p = [&](double s) { next = std::max(next, fabs(s * (a + s * s * (b + s * s * c)))); };
+    const auto see_b = [&](double u) { poly = std::max(poly, fabs(u * (b + c * u))); };
+    see_p(m);
+    see_b(t);
+    if (c != 0.0) {
+      const double d = 9.0 * b * b - 20.0 * a * c;
+      for (int sign = -1; sign <= 1 && d >= 0.0; sign += 2) {   // p' = a + 3 b s^2 + 5 c s^4
+        const double u = (-3.0 * b + sign * sqrt(d)) / (10.0 * c);
+        if (u > 0.0 && u < t) see_p(sqrt(u));
+      }
+      if (const double u = -b / (2.0 * c); u > 0.0 && u < t) see_b(u);
+    } else if (b != 0.0) {
+      if (const double u = -a / (3.0 * b); u > 0.0 && u < t) see_p(sqrt(u));
+    }
+    if (!(next < 1e30)) { m = next; if (i + 1 < steps) return false; break; }
+    m = next * margin;
+  }
+  const double largest[3] = {x, x * x, poly * margin};
+  for (int i = 0; i < 3; ++i) {
+    if (!(largest[i] <= kHalfMax)) return false;
+    int e = 15;
+    while (e > 0 && ldexp(largest[i], e) > kHalfMax) --e;
+    unit[i] = (float)(1 << e);
+  }
+  return true;
+}
+
 int ns_run(const char* fn, int n, const int64_t* batch, const int64_t* rows, const int64_t* cols, void* const* p,
            const int64_t* ldp, const int64_t* bsp, const void* const* g, const int64_t* ldg, const int64_t* bsg,
            float* const* m, const float* scale, int bf16, int prec, int steps, float a, float b, float c,
-           const NsStep& S, void* ws, int64_t ws_bytes, void* stream) {
+           NsStep S, void* ws, int64_t ws_bytes, void* stream) {
   MMS_REQUIRE(steps >= 1 && steps <= 64, fn, "1 to 64 steps");
   MMS_REQUIRE(S.eps > 0.0, fn, "eps must be positive");
+  MMS_REQUIRE(ns_units(steps, a, b, c, S.unit), fn,
+              "coefficients with which X, X X^T or b A + c A A can pass 60000 in fewer steps than these");
   MMS_REQUIRE(n == 0 || (p && ldp && bsp && g && ldg && bsg), fn, "null pointer table");
   const int rc = ns_check(fn, n, batch, rows, cols, prec);
   if (rc) return rc;
@@ -1028,7 +1094,7 @@ MMS_EXPORT int mms_muon_step(int n, const int64_t* batch, const int64_t* rows, c
   MMS_REQUIRE(n <= 0 || (m && scale), fn, "null momentum or scale table");
   MMS_REQUIRE(momentum >= 0.0 && momentum < 1.0, fn, "momentum must be in [0, 1)");
   for (int i = 0; i < n; ++i) MMS_REQUIRE(m[i] || !rows || !cols || !batch || batch[i] * rows[i] * cols[i] == 0, fn, "null momentum");
-  const NsStep S{(float)momentum, (float)(1.0 - momentum), nesterov, sumsq, max_norm, hyper, decay, neg_lr, eps};
+  const NsStep S{(float)momentum, (float)(1.0 - momentum), nesterov, sumsq, max_norm, hyper, decay, neg_lr, eps, {}};
   return ns_run(fn, n, batch, rows, cols, p, ldp, bsp, g, ldg, bsg, m, scale, bf16, prec, steps, a, b, c, S, ws,
                 ws_bytes, stream);
 }

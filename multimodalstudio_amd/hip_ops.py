@@ -305,7 +305,8 @@ def newton_schulz(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float
 
     ``mats``: a tensor [..., rows, cols] (a stack of matrices) or a list of such; float32 or bfloat16; returns the
     same structure, contiguous and without autograd history.  A zero matrix gives zeros, one with NaN or infinities NaN.
-    All matrices share the same few launches.
+    All matrices share the same few launches.  Coefficients with which a singular value of X before the last step, of A or
+    of b A + c A A can pass 60000 are refused.
 
     ``prec``: 0 (or None) fp32's accuracy whatever the type -- a bfloat16 result is off by its own rounding alone; 1
     bfloat16's accuracy for matrices of more than 128 rows and columns in about half of the time (8 x 1024 x 4096
@@ -350,7 +351,7 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
     ``params`` / ``grads``: lists of [..., rows, cols] tensors of one type each, float32 or bfloat16; ``momenta``:
     float32, contiguous, zeros before the first step.  ``sumsq`` (device, one float) with ``max_norm``: the gradients
     are clipped by min(1, max_norm / (sqrt(sumsq) + 1e-6)).  ``hyper`` (device): [1 - lr weight_decay, -lr] read by the
-    kernels in place of the arguments (graph replays).  ``prec``: as newton_schulz's."""
+    kernels in place of the arguments (graph replays).  ``coefficients``, ``prec``: as newton_schulz's."""
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise ValueError(f"muon_step: {len(params)} weights, {len(grads)} gradients, {len(momenta)} momenta")
