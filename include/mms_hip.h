@@ -479,6 +479,12 @@ int mms_adamw_dev_multi(int nseg, float* const* p, const float* const* g, float*
  * ws: mms_muon_workspace's bytes (HOST function), 256-byte aligned, used by this call alone while it runs. */
 int mms_muon_workspace(int n, const int64_t* batch, const int64_t* rows, const int64_t* cols, int prec,
                        int64_t* bytes);
+/* How a call of these matrices is launched (HOST function): *tables groups of matrices that share their launches, largest
+ * first, and of the first `max` groups six values each: the matrices, the fp16 values an operand's entry (2 with split
+ * fp16), the tiles' side for A, the 128-byte stages a block of A sums (0: all of a tile's), the sides for b A + c A A and
+ * for X. */
+int mms_muon_plan(int n, const int64_t* batch, const int64_t* rows, const int64_t* cols, int prec, int max,
+                  int64_t* plan, int64_t* tables);
 int mms_newton_schulz(int n, const int64_t* batch, const int64_t* rows, const int64_t* cols, const void* const* g,
                       const int64_t* ldg, const int64_t* bsg, void* const* out, const int64_t* ldo, const int64_t* bso,
                       int bf16, int prec, int steps, float a, float b, float c, double eps, void* ws, int64_t ws_bytes,

@@ -812,21 +812,28 @@ struct NsPlan {
 // 138; six of 701 x 1100, prec 0: A 20, 28, 46, 68 us, X 32, 33, 40, 54.
 // With `chunk`, tiles may be summed in parts of that many stages: as few parts as fill the card with one round of
 // blocks, and no more than the square root of the stages (a stage takes about as long as the adding of a part), where
-// that beats whole sums.  Parts cost 2 us, for their way through memory, and 0.3 for each that the last block adds.
+// that beats whole sums.  Parts cost 2 us, for their way through memory, and 0.3 for each that the last block adds.  Only
+// tiles up to 128 are split: with 256-wide ones a whole call was 9 .. 14% slower for it (2 x 501 x 991 with 2033 x 7973
+// prec 0: 2335 us, 2033 with the choice below), with 192-wide ones 7% faster to 4% slower.
 // prec 0: 64 x 4096 (128 stages) 38 us whole, 13 in 11 parts; 100 x 20000 (626) 177, 22 in 25 parts (29 in 53);
 // 300 x 4096 with 60 x 2000 and 1000 x 1000 40, 17.
 constexpr int kTiles[4] = {256, 192, 128, 64}, kPerCu[4] = {1, 1, 2, 3};
 constexpr float kGramCost[2][4] = {{1.90f, 1.22f, 0.55f, 0.23f}, {2.25f, 1.40f, 0.73f, 0.26f}};
 constexpr float kFullCost[2][4] = {{1.90f, 1.38f, 0.60f, 0.22f}, {2.00f, 1.38f, 0.62f, 0.21f}};
+// Estimates that come to the same go to the wider tile and to whole sums, not to a float's last bit: another tile has to
+// gain 0.1%, a split 5%, and 20% with 128-wide tiles of single fp16 operands, whose parts are the most traffic beside
+// their products (prec 1, a whole call, whole sums and split: 8 x 1024 x 4096 978 and 1050 us, 8 x 1071 x 8055 2216 and
+// 2310, 4 x 671 x 13842 1088 and 1043).
+constexpr float kTie = 0.999f, kSplit = 0.95f, kWideSplit = 0.8f;
 constexpr int kMinChunk = 12;
 template <typename Count, typename Stages>
-int choose_tile(int n, const float (&cost)[4], const Count& count, const Stages& stages, int* chunk) {
+int choose_tile(int n, int w, const float (&cost)[4], const Count& count, const Stages& stages, int* chunk) {
   int best = 64;
   float least = 1e30f;
   for (int k = 0; k < 4; ++k) {
     int64_t total = 0;
     int longest = 0;
-    for (int whole = 1; whole >= (chunk ? 0 : 1); --whole) {
+    for (int whole = 1; whole >= (chunk && kTiles[k] <= 128 ? 0 : 1); --whole) {
       int len = 1 << 30;
       if (!whole) {
         // the longest sum in equal parts, the others in parts of the same length
@@ -851,7 +858,7 @@ int choose_tile(int n, const float (&cost)[4], const Count& count, const Stages&
       }
       end = fmaxf(end, sum / 256);
       if (!whole && before > kMaxParts) continue;
-      if (end < least) {
+      if (end < least * (whole ? kTie : w == 1 && kTiles[k] > 64 ? kWideSplit : kSplit)) {
         least = end;
         best = kTiles[k];
         if (chunk) *chunk = len;
@@ -890,9 +897,9 @@ NsPlan plan_group(const int* order, int live, const int64_t* batch, const int64_
   const auto full = [&](int i, int t) { return full_blocks(layout(i), t) * batch[order[i]]; };
   const auto along = [&](int i) { return layout(i).cp * P.w / 64; };
   const auto across = [&](int i) { return layout(i).rp * P.w / 64; };
-  P.tiles.a = choose_tile(P.n, kGramCost[P.w - 1], gram, along, &P.tiles.chunk);
-  P.tiles.b = choose_tile(P.n, kGramCost[P.w - 1], gram, across, nullptr);
-  P.tiles.x = choose_tile(P.n, kFullCost[P.w - 1], full, across, nullptr);
+  P.tiles.a = choose_tile(P.n, P.w, kGramCost[P.w - 1], gram, along, &P.tiles.chunk);
+  P.tiles.b = choose_tile(P.n, P.w, kGramCost[P.w - 1], gram, across, nullptr);
+  P.tiles.x = choose_tile(P.n, P.w, kFullCost[P.w - 1], full, across, nullptr);
   bool split = false;
   for (int i = 0; i < P.n; ++i) {
     const int parts = gram_parts(layout(i), P.tiles.chunk);
@@ -1071,6 +1078,31 @@ MMS_EXPORT int mms_muon_workspace(int n, const int64_t* batch, const int64_t* ro
   NsPlan first;
   int64_t partial;
   *bytes = workspace_of(order, sort_matrices(n, batch, rows, cols, prec, order), batch, rows, cols, prec, first, partial);
+  return 0;
+}
+
+MMS_EXPORT int mms_muon_plan(int n, const int64_t* batch, const int64_t* rows, const int64_t* cols, int prec, int max,
+                             int64_t* plan, int64_t* tables) {
+  const char* fn = "mms_muon_plan";
+  MMS_REQUIRE(tables != nullptr && (plan != nullptr || max <= 0), fn, "null output");
+  const int rc = ns_check(fn, n, batch, rows, cols, prec);
+  if (rc) return rc;
+  static thread_local int order[kMaxMatrices];
+  const int live = sort_matrices(n, batch, rows, cols, prec, order);
+  *tables = 0;
+  for (int at = 0; at < live; ++*tables) {
+    const NsPlan P = plan_group(order + at, live - at, batch, rows, cols, prec);
+    if (*tables < max) {
+      int64_t* out = plan + 6 * *tables;
+      out[0] = P.n;
+      out[1] = P.w;
+      out[2] = P.tiles.a;
+      out[3] = P.partial ? P.tiles.chunk : 0;
+      out[4] = P.tiles.b;
+      out[5] = P.tiles.x;
+    }
+    at += P.n;
+  }
   return 0;
 }
 
