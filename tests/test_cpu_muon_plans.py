@@ -1,10 +1,14 @@
-"""How Newton-Schulz calls are launched (mms_muon_plan, a host function): a way is not left to a float's last bit."""
+"""How Newton-Schulz calls are launched (mms_muon_plan, a host function): the GPU tests take every way that ordinary sizes
+do, and a way is not left to a float's last bit."""
 from __future__ import annotations
 
 import ctypes
 import math
+import random
 
 import pytest
+
+from test_gpu_muon_plans import CASES
 
 
 @pytest.fixture(scope="module")
@@ -25,6 +29,39 @@ def plan(L, shapes, prec):
     out, tables = (ctypes.c_int64 * 48)(), ctypes.c_int64(-1)
     assert L.mms_muon_plan(*_tables(shapes), prec, 8, out, ctypes.addressof(tables)) == 0
     return [tuple(out[6 * i:6 * i + 6]) for i in range(tables.value)]
+
+
+def ways(L, shapes, prec):
+    """{(operands' width, product, tile, in parts)}, and the same for a matrix of at most 64 rows that shares them."""
+    found = set()
+    groups = plan(L, shapes, prec)
+    for n, w, a, chunk, b, x in groups:
+        kinds = {w}
+        if len(groups) == 1 and w == 2 and any(min(s[-2:]) <= 64 for s in shapes):
+            kinds.add("narrow")
+        for k in kinds:
+            found |= {(k, "A", a, chunk > 0), (k, "B", b, False), (k, "X", x, False)}
+    return found
+
+
+def test_gpu_tests_take_every_way(L):
+    tested = set()
+    for prec in (0, 1):
+        for shapes in CASES:
+            tested |= ways(L, shapes, prec)
+    rng = random.Random(3)
+
+    def log(lo, hi):
+        return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+    taken = {}
+    for _ in range(12000):
+        shapes = [(rng.choice([1, 1, 1, 2, 4, 8, 16, 32]), log(1, 6000), log(8, 12000)) for _ in range(rng.choice([1, 1, 1, 2, 3]))]
+        if sum(b * min(r, c) ** 2 * max(r, c) for b, r, c in shapes) <= 6e11:
+            for prec in (0, 1):
+                for w in ways(L, shapes, prec):
+                    taken.setdefault(w, (shapes, prec))
+    assert len(taken) >= 40
+    assert {w: s for w, s in taken.items() if w not in tested} == {}
 
 
 def test_equal_estimates_go_to_whole_sums(L):

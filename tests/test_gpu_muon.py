@@ -57,6 +57,7 @@ def gen(dev):
 DTYPES = [torch.float32, torch.bfloat16]
 # one row, one column, one value; below, at and over the tiles' sides; wide, tall, stacks; the three tile sizes (a
 # call's matrices use 128- and 256-wide tiles once they have 192 of them)
+# (That was the choice once.  Four tile sizes, by the expected end of the launch: test_gpu_muon_plans.py has them all.)
 SHAPES = [(1, 1), (1, 5), (5, 1), (1, 4097), (2, 2), (3, 64), (64, 64), (65, 63), (64, 257), (129, 128), (256, 71),
           (257, 256), (256, 317), (5, 100, 40), (2, 3, 33, 70), (4, 1000, 900), (13, 1024, 1030), (9, 1500, 1100)]
 
