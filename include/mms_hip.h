@@ -473,7 +473,8 @@ int mms_adamw_dev_multi(int nseg, float* const* p, const float* const* g, float*
  *   X = G / max(|G|_F, eps), then `steps` times X <- a X + (b A + c A A) X, A = X X^T, on the side with fewer rows.
  * Coefficients with which a singular value of an iterate before the last one, of A or of b A + c A A can pass 60000 are
  * refused (a, b, c = 3.4445, -4.7750, 2.0315 keep them below 3).  A matrix of zeros gives zeros; one with a NaN or
- * infinity gives NaN.
+ * infinity gives NaN.  What is written (out; p and m) must not overlap other matrices of the call, nor m its own p or g;
+ * such calls are refused.
  * prec 0: products of split fp16 (fp32's accuracy), 1: fp16 products where a matrix is large (bf16's accuracy), whatever
  * the matrices' type.
  * ws: mms_muon_workspace's bytes (HOST function), 256-byte aligned, used by this call alone while it runs. */

@@ -38,6 +38,7 @@
 #include "chain_common.h"
 
 #include <algorithm>
+#include <new>
 #include <type_traits>
 
 namespace {
@@ -1013,6 +1014,62 @@ bool ns_units(int steps, double a, double b, double c, float (&unit)[3]) {
   return true;
 }
 
+// ---- what a call writes may not be read or written by another of its matrices: their blocks run together ------------
+// Rows of `width` bytes, `ld` apart, in matrices `bs` apart, ascending and apart (of what is written: checked before).
+struct Rows {
+  uintptr_t lo, hi;      // first byte, past the last
+  int64_t width, ld, bs, rows, batch;
+  int matrix, kind;      // 0 gradients, 1 weights or results, 2 momenta
+};
+
+Rows rows_of(const void* p, int64_t es, int64_t rows, int64_t cols, int64_t ld, int64_t batch, int64_t bs, int matrix,
+             int kind) {
+  Rows r{(uintptr_t)p, 0, cols * es, rows > 1 ? ld * es : cols * es, batch > 1 ? bs * es : 0, rows, batch, matrix, kind};
+  r.hi = r.lo + (uintptr_t)((batch - 1) * r.bs + (rows - 1) * r.ld + r.width);
+  return r;
+}
+
+// does any row of `b` reach into [x, x + width)?
+bool reaches(const Rows& b, uintptr_t x, int64_t width) {
+  const int64_t y = (int64_t)(x - b.lo) + width - 1;   // the last byte, from b's first
+  if (y < 0) return false;
+  const int64_t k = b.batch > 1 ? std::min(y / b.bs, b.batch - 1) : 0, r = std::min((y - k * b.bs) / b.ld, b.rows - 1);
+  return k * b.bs + r * b.ld + b.width > y - width + 1;   // the last row that begins by then
+}
+
+bool overlap(const Rows& a, const Rows& b) {
+  if (a.hi <= b.lo || b.hi <= a.lo) return false;
+  const auto apart = [](const Rows& r) { return r.batch == 1 || r.bs >= (r.rows - 1) * r.ld + r.width; };
+  if (!apart(a) || !apart(b)) return true;   // a repeated gradient: not looked at row by row
+  const Rows &few = a.rows * a.batch <= b.rows * b.batch ? a : b, &many = &few == &a ? b : a;
+  // columns of one buffer, side by side
+  if (a.ld == b.ld && a.bs % a.ld == 0 && b.bs % a.ld == 0) {
+    const int64_t d = many.lo >= few.lo ? (int64_t)(many.lo - few.lo) % a.ld : (a.ld - (int64_t)(few.lo - many.lo) % a.ld) % a.ld;
+    if (d >= few.width && d + many.width <= a.ld) return false;
+  }
+  for (int64_t k = 0; k < few.batch; ++k)
+    for (int64_t r = 0; r < few.rows; ++r)
+      if (reaches(many, few.lo + (uintptr_t)(k * few.bs + r * few.ld), few.width)) return true;
+  return false;
+}
+
+// 0, or 1 if one of the call's matrices writes what another reads or writes, or its own momentum and weights or gradient
+// are not apart (a weight may lie where its own gradient does: that is read before).
+int conflict(Rows* all, int n) {
+  std::sort(all, all + n, [](const Rows& a, const Rows& b) { return a.lo < b.lo; });
+  uintptr_t reach = 0;   // of the rows before
+  for (int i = 0; i < n; ++i) {
+    if (all[i].lo < reach)
+      for (int j = 0; j < i; ++j) {
+        const Rows &a = all[i], &b = all[j];
+        if (a.kind + b.kind == 0 || (a.matrix == b.matrix && a.kind + b.kind == 1)) continue;
+        if (overlap(a, b)) return 1;
+      }
+    reach = std::max(reach, all[i].hi);
+  }
+  return 0;
+}
+
 int ns_run(const char* fn, int n, const int64_t* batch, const int64_t* rows, const int64_t* cols, void* const* p,
            const int64_t* ldp, const int64_t* bsp, const void* const* g, const int64_t* ldg, const int64_t* bsg,
            float* const* m, const float* scale, int bf16, int prec, int steps, float a, float b, float c,
@@ -1037,8 +1094,24 @@ int ns_run(const char* fn, int n, const int64_t* batch, const int64_t* rows, con
     MMS_REQUIRE(bsp[i] >= 0 && bsg[i] >= 0 && (batch[i] == 1 || bsp[i] >= rows[i] * ldp[i] - (ldp[i] - cols[i])), fn,
                 "stacked matrices must not overlap");
   }
-  MMS_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 255) == 0), fn,
-              "workspace too small (mms_muon_workspace) or not 256-byte aligned");
+  const char* small = "workspace too small (mms_muon_workspace) or not 256-byte aligned";
+  MMS_REQUIRE(need == 0 || ws, fn, small);
+  if (live) {
+    Rows* all = new (std::nothrow) Rows[3 * live];
+    MMS_REQUIRE(all != nullptr, fn, "out of host memory");
+    int count = 0;
+    const int64_t es = bf16 ? 2 : 4;
+    for (int k = 0; k < live; ++k) {
+      const int i = order[k];
+      all[count++] = rows_of(g[i], es, rows[i], cols[i], ldg[i], batch[i], bsg[i], i, 0);
+      all[count++] = rows_of(p[i], es, rows[i], cols[i], ldp[i], batch[i], bsp[i], i, 1);
+      if (m) all[count++] = rows_of(m[i], 4, rows[i], cols[i], cols[i], batch[i], rows[i] * cols[i], i, 2);
+    }
+    const int bad = conflict(all, count);
+    delete[] all;
+    MMS_REQUIRE(bad == 0, fn, "matrices that are written must not overlap others of the call");
+  }
+  MMS_REQUIRE(need == 0 || (ws_bytes >= need && ((uintptr_t)ws & 255) == 0), fn, small);
   hipStream_t s = mms::as_stream(stream);
   uint64_t* partial = (uint64_t*)ws;
   char* next = (char*)ws + parts;

@@ -349,7 +349,8 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
     p <- (1 - lr weight_decay) p - lr scale newton_schulz(u), scale = ``muon_scale(rows, cols, adjust)``.
 
     ``params`` / ``grads``: lists of [..., rows, cols] tensors of one type each, float32 or bfloat16; ``momenta``:
-    float32, contiguous, zeros before the first step.  ``sumsq`` (device, one float) with ``max_norm``: the gradients
+    float32, contiguous, zeros before the first step.  Weights or momenta that overlap others of the call are refused (a
+    list's types are stepped one after the other, each by itself).  ``sumsq`` (device, one float) with ``max_norm``: the gradients
     are clipped by min(1, max_norm / (sqrt(sumsq) + 1e-6)).  ``hyper`` (device): [1 - lr weight_decay, -lr] read by the
     kernels in place of the arguments (graph replays).  ``coefficients``, ``prec``: as newton_schulz's."""
     params, grads, momenta = list(params), list(grads), list(momenta)
