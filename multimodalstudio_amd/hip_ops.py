@@ -298,6 +298,11 @@ def _check_matrices(ts, what: str):
             raise ValueError(f"{what} must be on one device, got {device} and {t.device}")
 
 
+def _written(*ts: torch.Tensor):
+    """The kernels wrote these tensors: a backward pass that saved one of them before is to notice."""
+    torch.autograd.graph.increment_version(ts)
+
+
 def newton_schulz(mats, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7, prec: Optional[int] = None):
     """The nearest semi-orthogonal matrix, approximately, of each matrix by Newton-Schulz products:
     X = G / max(|G|_F, eps), then ``steps`` times X <- a X + (b A + c A A) X with A = X X^T (X^T X for tall G) -- the
@@ -396,6 +401,7 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
                       bf16, prec, int(steps), a, b, c, float(eps), float(momentum), int(bool(nesterov)), _ptr(sumsq),
                       float(max_norm), _ptr(hyper), 1.0 - float(lr) * float(weight_decay), -float(lr), ws.data_ptr(),
                       ws.numel(), _stream_of(params[0]))
+        _written(*(params[i] for i in pick), *(momenta[i] for i in pick))
 
 
 # ----------------------------------------------------------------------------------------------
@@ -489,6 +495,7 @@ def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: 
         _lib.call("mms_embedding_bwd", flat.data_ptr(), ids.dtype is torch.int64, stride, n, d.data_ptr(),
                   dim if n <= 1 else d.stride(0), rows, dim, dt, scale, pad, out.data_ptr(),
                   dim if rows == 1 else out.stride(0), bool(accumulate), _ptr(ws), need, _stream_of(dout))
+    _written(out)
     return out
 
 

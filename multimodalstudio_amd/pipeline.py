@@ -234,7 +234,7 @@ class MuonGroup(FlatGroup):
 
     def update(self, max_norm: float, **scalars):
         """The Muon launches on the gradients and their sum of squares."""
-        hip_ops.muon_step([p.data for p in self.params], [p.grad for p in self.params], self.momenta,
+        hip_ops.muon_step(self.params, [p.grad for p in self.params], self.momenta,
                           momentum=self.momentum, nesterov=self.nesterov, steps=self.steps,
                           coefficients=self.coefficients, eps=self.eps, adjust=self.adjust, sumsq=self.sumsq,
                           max_norm=float(max_norm), **scalars)

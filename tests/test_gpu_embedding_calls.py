@@ -1,0 +1,26 @@
+"""Calls of the row tables' operators beside the plain ones of test_gpu_embedding.py: what they write, and what they
+refuse to."""
+import pytest
+import torch
+
+from test_gpu_embedding import check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture()
+def gen(dev):
+    return torch.Generator(device="cuda").manual_seed(61)
+
+
+@pytest.mark.parametrize("n", [100, 1000])
+def test_backward_passes_notice_the_gradient_written_into_a_tensor(dev, gen, n):
+    from multimodalstudio_amd import hip_ops
+    ids = torch.randint(0, 300, (n,), device="cuda", generator=gen)
+    dout, out = torch.randn(n, 16, device="cuda", generator=gen), torch.randn(300, 16, device="cuda", generator=gen)
+    w = torch.randn(300, 16, device="cuda", generator=gen, requires_grad=True)
+    loss = (out * w).sum()
+    hip_ops.embedding_backward(ids, dout, 300, out=out)
+    check(out, ids, dout, 300)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()

@@ -30,6 +30,27 @@ def test_overlapping_matrices(dev, gen):
     assert all(torch.equal(a, b) for a, b in zip((w, g, m, stack), keep))
 
 
+def test_backward_passes_notice_the_step(dev, gen):
+    """A backward pass that saved the weights or a momentum from before the step raises instead of using the new ones."""
+    from multimodalstudio_amd import hip_ops
+    from multimodalstudio_amd import pipeline as pl
+    x = torch.randn(5, 8, device="cuda", generator=gen, requires_grad=True)
+    p, g = torch.nn.Parameter(torch.randn(6, 8, device="cuda", generator=gen)), torch.randn(6, 8, device="cuda", generator=gen)
+    m = torch.zeros(6, 8, device="cuda")
+    for saved in (p, m):
+        loss = (x @ saved.mT).sum()
+        hip_ops.muon_step([p], [g], [m], lr=0.1)
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+    group = pl.MuonGroup([p], lr=0.1, weight_decay=0.0)
+    p.grad.copy_(g)
+    loss = (x @ p.mT).sum()
+    group.step(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    assert p.grad.data_ptr() == group.grad.data_ptr() and p.data_ptr() == group.flat.data_ptr()
+
+
 def test_columns_side_by_side(dev, gen):
     """Weights that are columns of one buffer, as fused projections are, each stepped by itself."""
     from multimodalstudio_amd import hip_ops
