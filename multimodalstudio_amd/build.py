@@ -36,13 +36,18 @@ CFLAGS = [
 
 def _compile(src: Path) -> Path:
     obj = BUILD / (src.stem + ".o")
-    deps = [src] + sorted(CSRC.glob("*.h")) + sorted(INCLUDE.glob("*.h"))
-    if obj.exists() and all(obj.stat().st_mtime >= d.stat().st_mtime for d in deps):
-        return obj
     cmd = [HIPCC, *CFLAGS, "-c", str(src), "-o", str(obj)]
+    # the command an object was compiled with lies beside it: another compiler, target or flag compiles it again
+    used = BUILD / (src.stem + ".cmd")
+    deps = [src] + sorted(CSRC.glob("*.h")) + sorted(INCLUDE.glob("*.h"))
+    if obj.exists() and used.exists() and used.read_text() == "\n".join(cmd) and \
+            all(obj.stat().st_mtime >= d.stat().st_mtime for d in deps):
+        return obj
+    used.unlink(missing_ok=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc failed for {src.name}:\n{res.stdout}\n{res.stderr}")
+    used.write_text("\n".join(cmd))
     return obj
 
 
