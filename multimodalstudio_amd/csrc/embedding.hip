@@ -78,7 +78,7 @@ __device__ __forceinline__ uint32_t key_at(const Ids& I, int64_t i) {
 
 // ---- lookup -------------------------------------------------------------------------------------------------------
 // A team of `lanes` threads (a power of two, at most 256) per R rows' segments of lanes pieces; blockIdx.y: the segment.
-template <typename T, bool WHOLE, int R>
+template <typename T, bool WHOLE, int R, bool STREAM>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(Ids I, int64_t n, const T* __restrict__ table, int64_t ldt,
                                                             int dim, int lanes_log2, float scale, T* __restrict__ out,
                                                             int64_t ldo) {
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(Ids I, int64_t n, co
       asm("" : "+v"(y));   // rounded to fp32 before fp16 (not v_fma_mixlo's one rounding): the bits of the same product in torch
       x[r].v[q] = (T)y;
     }
-    store_piece<WHOLE, (R > 1)>(out + (i0 + r) * ldo + c, x[r], dim - c);
+    store_piece<WHOLE, STREAM>(out + (i0 + r) * ldo + c, x[r], dim - c);
   }
 }
 
@@ -799,14 +799,21 @@ template <typename T>
 void launch_fwd(const Ids& I, int64_t n, const void* table, int64_t ldt, int dim, float scale, void* out, int64_t ldo,
                 hipStream_t s) {
   constexpr int N = Piece<T>::N;
-  // 4 rows a team, past the caches, once there are blocks enough (33 MB of output; 16384 x 4096 bf16: 46 us with one row
-  // a team, 42 with 4, 32 past the caches)
+  // 4 rows a team once there are blocks enough (33 MB of output; 16384 x 4096 bf16: 46 us with one row a team, 42 with 4);
+  // past the caches from half of the last one on.  That alone is faster always (16384 x 4096: 32 us), but what reads the
+  // rows next pays for it: lookup and a product with a 4096 x 256 matrix, through the caches and past them, 64 MB of rows
+  // 63.6 and 66.4 us, 128 MB 91 and 94, 256 MB 185 and 163; lookup and an elementwise pass 41.9 and 43.2, 90.5 and 84.5,
+  // 177 and 174.
   const int l = lanes_for(dim, N), segs = (dim + (N << l) - 1) / (N << l);
   const bool many = (n << l) * segs >= 4 * 256 * 2048;
   const int per = (256 >> l) * (many ? 4 : 1);
   const dim3 grid((unsigned)((n + per - 1) / per), (unsigned)segs);
-  const auto kernel = dim % N == 0 ? many ? embedding_fwd_kernel<T, true, 4> : embedding_fwd_kernel<T, true, 1>
-                                   : many ? embedding_fwd_kernel<T, false, 4> : embedding_fwd_kernel<T, false, 1>;
+  const bool stream = many && n * dim * (int64_t)sizeof(T) >= kLargeTable;
+  const auto kernel =
+      dim % N == 0 ? stream ? embedding_fwd_kernel<T, true, 4, true> : many ? embedding_fwd_kernel<T, true, 4, false>
+                                                                            : embedding_fwd_kernel<T, true, 1, false>
+                   : stream ? embedding_fwd_kernel<T, false, 4, true> : many ? embedding_fwd_kernel<T, false, 4, false>
+                                                                             : embedding_fwd_kernel<T, false, 1, false>;
   hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, I, n, (const T*)table, ldt, dim, l, scale, (T*)out, ldo);
 }
 

@@ -24,3 +24,15 @@ def test_backward_passes_notice_the_gradient_written_into_a_tensor(dev, gen, n):
     check(out, ids, dout, 300)
     with pytest.raises(RuntimeError, match="inplace"):
         loss.backward()
+
+
+@pytest.mark.parametrize("n,dim", [(9000, 1025), (20000, 1024), (70000, 1024), (70001, 1027)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_lookups_through_the_caches_and_past_them(dev, gen, n, dim, dtype):
+    """Outputs below 33 MB, between that and 128 MB, and larger ones, rows of whole pieces and others."""
+    from multimodalstudio_amd import hip_ops
+    table = torch.randn(700, dim, device="cuda", generator=gen).to(dtype)
+    ids = torch.randint(-2, 703, (n,), device="cuda", generator=gen)
+    want = (table[ids.clamp(0, 699)].float() * 0.3).to(dtype)
+    want[(ids < 0) | (ids >= 700)] = 0
+    assert torch.equal(hip_ops.embedding(ids, table, 0.3), want)
