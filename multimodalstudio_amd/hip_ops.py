@@ -408,6 +408,7 @@ def muon_step(params, grads, momenta, lr: float, momentum: float = 0.95, nestero
 # learned row tables
 # ----------------------------------------------------------------------------------------------
 _TABLE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_MAX_INDICES = (1 << 24) - 1      # of one mms_embedding_* call
 
 
 def _check_table(ids: torch.Tensor, rows: torch.Tensor, what: str) -> int:
@@ -448,9 +449,12 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> tor
     t = table if table.is_contiguous() or (table.stride(1) == 1 and table.stride(0) >= dim) else table.contiguous()
     out = torch.empty(*ids.shape, dim, dtype=table.dtype, device=table.device)
     flat, stride = _flat_ids(ids)
+    n = ids.numel()
     with _on_device(t):
-        _lib.call("mms_embedding_fwd", flat.data_ptr(), ids.dtype is torch.int64, stride, ids.numel(), t.data_ptr(),
-                  dim if rows == 1 else t.stride(0), rows, dim, dt, scale, out.data_ptr(), dim, _stream_of(t))
+        for i in range(0, n, _MAX_INDICES):
+            _lib.call("mms_embedding_fwd", flat.data_ptr() + i * stride * ids.element_size(), ids.dtype is torch.int64,
+                      stride, min(n - i, _MAX_INDICES), t.data_ptr(), dim if rows == 1 else t.stride(0), rows, dim, dt,
+                      scale, out.data_ptr() + i * dim * t.element_size(), dim, _stream_of(t))
     return out
 
 
@@ -467,7 +471,7 @@ def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: 
     """The table's gradient [rows, dim] in ``dout``'s type: scale * the sum of dout over the positions of each row, in
     fp32 and in an order that ``ids`` alone fixes (the same bits on each call).  Positions whose index is
     ``padding_idx`` or outside the table add nothing, whatever ``dout`` holds there.  ``out``: written in place, or
-    added into with ``accumulate``."""
+    added into with ``accumulate``.  At most 2^24 - 1 positions (more: in parts, with ``accumulate``)."""
     dt = _check_table(ids, dout, "the gradient")
     dim = dout.shape[-1] if dout.dim() else 0
     if dim == 0 or dout.shape[:-1] != ids.shape or rows < 1:
@@ -501,10 +505,12 @@ def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: 
 
 class EmbeddingFunction(torch.autograd.Function):
     """Learned row table forward / backward on the HIP kernels: apply(ids, table, scale=1.0, padding_idx=None).  Once
-    differentiable: a derivative of its gradient raises."""
+    differentiable: a derivative of its gradient raises.  At most 2^24 - 1 indices where the table wants a gradient."""
 
     @staticmethod
     def forward(ctx, ids, table, scale: float = 1.0, padding_idx: Optional[int] = None):
+        if ctx.needs_input_grad[1] and ids.numel() > _MAX_INDICES:
+            raise ValueError(f"EmbeddingFunction: {ids.numel()} indices, the gradient takes up to {_MAX_INDICES}")
         ctx.save_for_backward(ids)
         ctx.cfg = (table.shape[0], float(scale), padding_idx)
         return embedding(ids, table, scale)

@@ -36,3 +36,22 @@ def test_lookups_through_the_caches_and_past_them(dev, gen, n, dim, dtype):
     want = (table[ids.clamp(0, 699)].float() * 0.3).to(dtype)
     want[(ids < 0) | (ids >= 700)] = 0
     assert torch.equal(hip_ops.embedding(ids, table, 0.3), want)
+
+
+@pytest.mark.parametrize("column", [False, True])
+def test_lookups_of_more_than_2_to_24_indices(dev, gen, column):
+    from multimodalstudio_amd import hip_ops
+    n = 2 ** 24 + 77
+    coords = torch.randint(-1, 60, (n, 2), device="cuda", generator=gen, dtype=torch.int32)
+    ids = coords[:, 1] if column else coords[:, 1].contiguous()
+    table = torch.randn(59, 3, device="cuda", generator=gen).half()
+    out = hip_ops.embedding(ids, table, 1.5)
+    want = (table[ids.clamp(0, 58).long()].float() * 1.5).half()
+    want[(ids < 0) | (ids >= 59)] = 0
+    assert torch.equal(out, want)
+    # the gradient sorts at most 2^24 - 1 positions: refused before the forward pass, not after it
+    with pytest.raises(ValueError, match="indices"):
+        hip_ops.EmbeddingFunction.apply(ids, table.requires_grad_())
+    assert hip_ops.EmbeddingFunction.apply(ids, table.detach()).shape == (n, 3)
+    with pytest.raises(RuntimeError, match="indices"):
+        hip_ops.embedding_backward(ids, out, 59)
