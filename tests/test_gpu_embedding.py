@@ -57,6 +57,7 @@ def draw_ids(kind, n, rows, gen):
 
 # n: none, around a run's length, a one-block sort's end (12288), several blocks, more than 64 of them; rows: one and
 # two sort digits and their borders, three digits; dim: one value, below / over 16 bytes, one and more column segments
+# (One block sorts up to 4096 positions, of tables of 65 rows and more; test_gpu_embedding_calls.py has its ends.)
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("n,rows,dim,kind", [
     (0, 7, 8, "uniform"), (1, 1, 1, "same"), (1, 5, 4100, "uniform"), (2, 2, 3, "reversed"), (63, 9, 16, "uniform"),

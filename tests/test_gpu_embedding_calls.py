@@ -3,7 +3,7 @@ refuse to."""
 import pytest
 import torch
 
-from test_gpu_embedding import check
+from test_gpu_embedding import check, draw_ids
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +55,27 @@ def test_lookups_of_more_than_2_to_24_indices(dev, gen, column):
     assert hip_ops.EmbeddingFunction.apply(ids, table.detach()).shape == (n, 3)
     with pytest.raises(RuntimeError, match="indices"):
         hip_ops.embedding_backward(ids, out, 59)
+
+
+# A sort by one block (129 .. 4096 positions) in one, two and three digits of the row: 1023 rows are one digit's last,
+# 2^20 - 1 two digits'; its ends, one position more (several blocks), some positions beside its 64-lane rounds
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("n,rows,dim", [
+    (129, 1023, 40), (129, 50257, 33), (1024, 1024, 40), (1025, 32000, 130), (2047, 32000, 7), (2500, 1048575, 3),
+    (2500, 1048576, 3), (3000, 2097153, 2), (4095, 131072, 8), (4096, 131072, 8), (4097, 131072, 8), (4096, 1025, 771),
+])
+@pytest.mark.parametrize("kind", ["uniform", "skewed", "outside", "same", "reversed"])
+def test_one_block_sort(dev, gen, n, rows, dim, dtype, kind):
+    from multimodalstudio_amd import hip_ops
+    ids = draw_ids(kind, n, rows, gen)
+    dout = torch.randn(n, dim, device="cuda", generator=gen).to(dtype)
+    got = hip_ops.embedding_backward(ids, dout, rows, 0.6)
+    check(got, ids, dout, rows, 0.6)
+    assert torch.equal(got, hip_ops.embedding_backward(ids.int(), dout, rows, 0.6))
+    # padding that holds what must reach nothing, into columns of a wider buffer
+    pad = int(ids[n // 3].clamp(0, rows - 1))
+    dirty = torch.where((ids == pad)[:, None], torch.full((), float("nan"), dtype=dtype, device="cuda"), dout)
+    buf = torch.full((rows, dim + 5), 7.0, dtype=dtype, device="cuda")
+    hip_ops.embedding_backward(ids, dirty, rows, 0.6, padding_idx=pad, out=buf[:, 2:2 + dim])
+    check(buf[:, 2:2 + dim], ids, torch.nan_to_num(dirty, 0.0), rows, 0.6, pad)
+    assert (buf[:, :2] == 7).all() and (buf[:, 2 + dim:] == 7).all()
