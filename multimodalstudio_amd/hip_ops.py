@@ -458,6 +458,24 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> tor
     return out
 
 
+def _rows_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Do two tensors of rows [..., dim] share memory?  Columns of one buffer, side by side, do not; rows of different
+    strides whose ranges meet count as if they did."""
+    if a.numel() == 0 or b.numel() == 0 or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+        return False
+
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + (sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    if a.dim() != 2 or b.dim() != 2 or a.stride(0) != b.stride(0) or a.stride(1) != 1 or b.stride(1) != 1 or a.stride(0) == 0:
+        return True
+    es = a.element_size()
+    ld, d = a.stride(0) * es, (b0 - a0) % (a.stride(0) * es)
+    return not (d >= a.shape[1] * es and d + b.shape[1] * es <= ld)
+
+
 @functools.lru_cache(maxsize=256)
 def _embedding_workspace(n: int, rows: int, dim: int, dt: int) -> int:
     need = ctypes.c_int64(0)
@@ -485,6 +503,8 @@ def embedding_backward(ids: torch.Tensor, dout: torch.Tensor, rows: int, scale: 
             (dim > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < dim):
         raise ValueError(f"embedding_backward: out must be [{rows}, {dim}] {dout.dtype} with contiguous rows on "
                          f"{dout.device}")
+    elif _rows_overlap(out, dout):
+        raise ValueError("embedding_backward: out must not share memory with the gradient it is the sum of")
     pad = -1
     if padding_idx is not None:
         if not -rows <= padding_idx < rows:

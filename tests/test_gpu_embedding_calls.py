@@ -79,3 +79,20 @@ def test_one_block_sort(dev, gen, n, rows, dim, dtype, kind):
     hip_ops.embedding_backward(ids, dirty, rows, 0.6, padding_idx=pad, out=buf[:, 2:2 + dim])
     check(buf[:, 2:2 + dim], ids, torch.nan_to_num(dirty, 0.0), rows, 0.6, pad)
     assert (buf[:, :2] == 7).all() and (buf[:, 2 + dim:] == 7).all()
+
+
+@pytest.mark.parametrize("n", [100, 600])
+def test_gradient_written_where_it_is_read(dev, gen, n):
+    """Refused; into other columns of the same buffer it is right."""
+    from multimodalstudio_amd import hip_ops
+    buf = torch.randn(n, 48, device="cuda", generator=gen)
+    ids = torch.randint(0, n, (n,), device="cuda", generator=gen)
+    keep = buf.clone()
+    for dout, out in ((buf, buf), (buf[:, :20], buf[:, 19:39])):
+        for accumulate in (False, True):
+            with pytest.raises(ValueError, match="share"):
+                hip_ops.embedding_backward(ids, dout, n, out=out, accumulate=accumulate)
+    assert torch.equal(buf, keep)
+    hip_ops.embedding_backward(ids, buf[:, :20], n, out=buf[:, 20:40])
+    check(buf[:, 20:40], ids, keep[:, :20], n)
+    assert torch.equal(buf[:, :20], keep[:, :20]) and torch.equal(buf[:, 40:], keep[:, 40:])
