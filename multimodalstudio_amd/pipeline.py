@@ -130,6 +130,7 @@ class FlatGroup:
         self.m = torch.zeros(n + pad, device=dev)
         self.v = torch.zeros(n + pad, device=dev)
         self.sumsq = torch.zeros(1, device=dev)
+        self.norm_groups: Optional[List[FlatGroup]] = None   # whose gradients' norm the clip goes by, if not its own's
         # this step's AdamW scalars for graph replays (mms_adamw_dev; layout of mms_adamw_scalars)
         self.hyper = torch.zeros(8, device=dev)
         # two pinned staging buffers, alternated: a step's scalars can be queued behind the previous replay while
@@ -170,12 +171,17 @@ class FlatGroup:
         self.step_count += 1
         return self.lr * lr_factor
 
+    def sumsq_of_grads(self):
+        """The sum of squares that the clip goes by."""
+        self.sumsq.zero_()
+        for g in self.norm_groups or [self]:
+            g.check_grads_attached()
+            _lib.call("mms_sumsq", g.grad.data_ptr(), g.n, self.sumsq.data_ptr(), _s())
+
     def step(self, lr_factor: float, max_norm: float = 2.0):
         """clip_grad_norm_(max_norm) then torch AdamW math (single launch each; scalars stay on device)."""
-        self.check_grads_attached()
         lr = self._advance(lr_factor)
-        self.sumsq.zero_()
-        _lib.call("mms_sumsq", self.grad.data_ptr(), self.n, self.sumsq.data_ptr(), _s())
+        self.sumsq_of_grads()
         _lib.call("mms_adamw", self.flat.data_ptr(), self.grad.data_ptr(), self.m.data_ptr(), self.v.data_ptr(), self.n,
                   self.sumsq.data_ptr(), float(max_norm), float(lr), float(self.wd), float(self.betas[0]),
                   float(self.betas[1]), float(self.eps), int(self.step_count), _s())
@@ -195,17 +201,23 @@ class FlatGroup:
 
     def step_captured(self, max_norm: float = 2.0):
         """The clip + AdamW launches with device-resident scalars (captured into the step graph)."""
-        self.check_grads_attached()
-        self.sumsq.zero_()
-        _lib.call("mms_sumsq", self.grad.data_ptr(), self.n, self.sumsq.data_ptr(), _s())
+        self.sumsq_of_grads()
         _lib.call("mms_adamw_dev", self.flat.data_ptr(), self.grad.data_ptr(), self.m.data_ptr(), self.v.data_ptr(),
                   self.n, self.sumsq.data_ptr(), float(max_norm), self.hyper.data_ptr(), _s())
 
 
+def clip_together(groups: Sequence["FlatGroup"]) -> None:
+    """One clip for several groups: each goes by the norm of all their gradients, as clip_grad_norm_ over their
+    parameters (before an OptimBank is made of them)."""
+    for g in groups:
+        g.sumsq, g.norm_groups = groups[0].sumsq, list(groups)
+
+
 class MuonGroup(FlatGroup):
-    """Weight matrices stepped by Muon (hip_ops.muon_step) in place of AdamW: the same flat buffers, clip and schedule;
-    ``m`` is the momentum and there is no second moment.  The learning rate's factor per matrix is
-    ``hip_ops.muon_scale``: with "match_rms_adamw" an AdamW group's lr and weight_decay carry over."""
+    """Weight matrices stepped by Muon (hip_ops.muon_step) in place of AdamW: the same flat buffers, schedule and clip (by
+    this group's own norm, or by that of several groups: clip_together); ``m`` is the momentum and there is no second
+    moment.  The learning rate's factor per matrix is ``hip_ops.muon_scale``: with "match_rms_adamw" an AdamW group's lr
+    and weight_decay carry over."""
 
     def __init__(self, params: List[nn.Parameter], lr: float, weight_decay: float, momentum: float = 0.95,
                  nesterov: bool = True, steps: int = 5, coefficients=hip_ops.NS_COEFFICIENTS, eps: float = 1e-7,
@@ -227,17 +239,12 @@ class MuonGroup(FlatGroup):
         self.sumsq_of_grads()
         self.update(max_norm, **scalars)
 
-    def sumsq_of_grads(self):
-        self.check_grads_attached()
-        self.sumsq.zero_()
-        _lib.call("mms_sumsq", self.grad.data_ptr(), self.n, self.sumsq.data_ptr(), _s())
-
     def update(self, max_norm: float, **scalars):
         """The Muon launches on the gradients and their sum of squares."""
         hip_ops.muon_step(self.params, [p.grad for p in self.params], self.momenta,
                           momentum=self.momentum, nesterov=self.nesterov, steps=self.steps,
-                          coefficients=self.coefficients, eps=self.eps, adjust=self.adjust, sumsq=self.sumsq,
-                          max_norm=float(max_norm), **scalars)
+                          coefficients=self.coefficients, eps=self.eps, adjust=self.adjust,
+                          sumsq=self.sumsq if max_norm > 0.0 else None, max_norm=float(max_norm), **scalars)
 
     def step(self, lr_factor: float, max_norm: float = 2.0):
         """clip_grad_norm_(max_norm) then the Muon step."""
@@ -266,6 +273,8 @@ class OptimBank:
         G = len(self.groups)
         if not 1 <= G <= 4:
             raise ValueError("OptimBank holds 1 to 4 groups")
+        if any(all(h is not k for k in self.groups) for g in self.groups for h in g.norm_groups or []):
+            raise ValueError("OptimBank: a group is clipped together with one that is not in the bank")
         dev = self.groups[0].flat.device
         self.hyper = torch.zeros(G * 8, device=dev)
         for i, g in enumerate(self.groups):
@@ -592,6 +601,8 @@ class Trainer:
         rest = [p for p in self.model.parameters() if not any(p is q for q in mats)]
         self.fields = FlatGroup(rest, lr=1e-3, weight_decay=0.01, eps=1e-15)
         self.matrices = MuonGroup(mats, lr=1e-3, weight_decay=0.01) if mats else None
+        if self.matrices is not None:
+            clip_together([self.fields, self.matrices])     # the fields' gradients, as with AdamW for all of them
         pose_params = list(self.pose.parameters())
         self.poses = FlatGroup(pose_params, lr=1e-4, weight_decay=0.01, eps=1e-15) if pose_params else None
         self.groups = [g for g in (self.fields, self.matrices, self.poses) if g is not None]

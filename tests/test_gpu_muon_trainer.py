@@ -1,0 +1,87 @@
+"""Muon in the trainer: one clip over all of the fields' gradients, and replayed steps that move the matrices as eager
+ones do."""
+import pytest
+import torch
+
+from test_gpu_muon import check_step, reference_step
+
+pytestmark = pytest.mark.gpu
+
+
+def _groups(dev, together):
+    from multimodalstudio_amd import pipeline as pl
+    gen = torch.Generator().manual_seed(6)
+    mats = [torch.nn.Parameter((0.1 * torch.randn(s, generator=gen)).to(dev)) for s in ((60, 71), (33, 60))]
+    vec = torch.nn.Parameter(torch.randn(500, generator=gen).to(dev))
+    ad = pl.FlatGroup([vec], lr=1e-3, weight_decay=0.01, eps=1e-15)
+    mu = pl.MuonGroup(mats, lr=1e-2, weight_decay=0.1)
+    if together:
+        pl.clip_together([ad, mu])
+    return ad, mu, vec, mats
+
+
+@pytest.mark.parametrize("form", ["eager", "captured", "bank"])
+@pytest.mark.parametrize("together", [True, False])
+def test_clip_of_several_groups(dev, form, together):
+    """Gradients of norms 4 and 3: clipped at 2 together by 2 / 5, each by itself by 2 / 4 and 2 / 3."""
+    from multimodalstudio_amd import pipeline as pl
+    ad, mu, vec, mats = _groups(dev, together)
+    bank = pl.OptimBank([ad, mu]) if form == "bank" else None
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    ref = vec.detach().clone().requires_grad_()
+    adamw = torch.optim.AdamW([ref], lr=1e-3, weight_decay=0.01, eps=1e-15)
+    for t in range(2):
+        if bank:
+            bank.zero_grads()
+        else:
+            ad.zero_grad()
+            mu.zero_grad()
+        for group, norm in ((ad, 4.0), (mu, 3.0)):
+            group.grad[:group.n].normal_(generator=gen)
+            group.grad.mul_(norm / group.grad.norm())
+        clip = {True: (0.4, 0.4), False: (0.5, 2.0 / 3.0)}[together]
+        want = [reference_step(p.detach(), p.grad, m, 1e-2, 0.95, True, 0.1, "match_rms_adamw", clip[1])
+                for p, m in zip(mats, mu.momenta)]
+        ref.grad = vec.grad * clip[0]
+        adamw.step()
+        if bank:
+            bank.load_hyper(1.0)
+            bank.step_captured()
+        else:
+            for g in (ad, mu):
+                if form == "captured":
+                    g.load_hyper(1.0)
+                    g.step_captured()
+                else:
+                    g.step(1.0)
+        for p, m, w in zip(mats, mu.momenta, want):
+            # the norm is a float32 sum of 6743 squares by atomics and a quotient: some half steps on the momentum
+            assert float((m.double() - w[1]).norm()) <= 64 * 2.0 ** -24 * float(w[1].norm())
+            check_step(p.detach(), w[1].float(), w, torch.float32)
+        assert (vec - ref).abs().max() <= 2e-6 * ref.abs().max()
+
+
+def test_no_clip_and_a_torn_bank(dev):
+    """max_norm 0 does not clip, as with AdamW; a bank needs every group that the clip goes by."""
+    from multimodalstudio_amd import pipeline as pl
+    ad, mu, vec, mats = _groups(dev, True)
+    mu.grad.fill_(1.0)
+    want = [reference_step(p.detach(), p.grad, m, 1e-2, 0.95, True, 0.1, "match_rms_adamw") for p, m in zip(mats, mu.momenta)]
+    mu.step(1.0, max_norm=0.0)
+    for p, m, w in zip(mats, mu.momenta, want):
+        check_step(p.detach(), m, w, torch.float32)
+    with pytest.raises(ValueError, match="bank"):
+        pl.OptimBank([mu])
+
+
+def test_the_trainer_clips_as_with_adamw(dev):
+    from multimodalstudio_amd import pipeline as pl
+    cfg = pl.TrainConfig(num_rays_per_modality=64, log2T=12, width=64, height=48, n_views=20, optimizer="muon")
+    t = pl.Trainer(cfg, dev)
+    assert t.fields.norm_groups == [t.fields, t.matrices] == t.matrices.norm_groups and t.poses.norm_groups is None
+    assert t.fields.sumsq is t.matrices.sumsq and t.poses.sumsq is not t.fields.sumsq
+    t.set_step(9500)
+    t.train_step()
+    total = sum(float(g.grad.double().square().sum()) for g in (t.fields, t.matrices))
+    # a float32 sum of 10^5 .. 10^6 squares, by blocks and atomics
+    assert abs(float(t.fields.sumsq) - total) <= 1e-4 * total
