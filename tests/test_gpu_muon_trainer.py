@@ -85,3 +85,44 @@ def test_the_trainer_clips_as_with_adamw(dev):
     total = sum(float(g.grad.double().square().sum()) for g in (t.fields, t.matrices))
     # a float32 sum of 10^5 .. 10^6 squares, by blocks and atomics
     assert abs(float(t.fields.sumsq) - total) <= 1e-4 * total
+
+
+def test_replayed_steps_move_the_matrices_as_eager_ones(dev):
+    """Each step of a GraphTrainer, its eager first one and the replays, moves the matrices as the definition does on the
+    gradients that the step left, clipped by the fields' norm; and the losses follow those of eager steps from the same
+    state (within the 1e-3 that test_gpu_graph.py has for float-atomic gradients)."""
+    from multimodalstudio_amd import graphs
+    from multimodalstudio_amd import pipeline as pl
+    cfg = pl.TrainConfig(method="grid", modalities=("rgb",), num_rays_per_modality=512, log2T=14, n_views=10, width=160,
+                         height=128, optimizer="muon")
+
+    def make():
+        t = pl.Trainer(cfg, dev)
+        t.set_step(95000)
+        t.model.eval()       # no sampler jitter: both see the same samples
+        return t
+    eager, t = make(), make()
+    runner = graphs.GraphTrainer(t, granule=64)
+    losses = []
+    for k in range(6):
+        before = [p.detach().clone() for p in t.matrices.params]
+        momenta = [m.clone() for m in t.matrices.momenta]
+        lr = 1e-3 * pl.lr_factor(t.step, cfg.max_iters)
+        replays = runner.stats["replays"]
+        losses.append((float(eager.train_step()[1]), float(runner.step()[1])))
+        torch.cuda.synchronize()
+        assert k < 2 or runner.stats["replays"] == replays + 1, (k, runner.stats)
+        total = sum(float(g.grad.double().square().sum()) for g in (t.fields, t.matrices))
+        clip = min(1.0, 2.0 / (total ** 0.5 + 1e-6))
+        moved = 0.0
+        for p, q, m, n in zip(before, t.matrices.params, momenta, t.matrices.momenta):
+            want = reference_step(p, q.grad, m, lr, 0.95, True, 0.01, "match_rms_adamw", clip)
+            # the clip goes by a float32 sum of 10^5 .. 10^6 squares
+            assert float((n.double() - want[1]).norm()) <= 1e-4 * float(want[1].norm())
+            check_step(q.detach(), want[1].float(), want, torch.float32)
+            moved += float((q.detach() - p).norm())
+        assert moved > 0.0
+    assert runner.disabled is None and runner.stats["replays"] >= 4
+    assert t.matrices.step_count == t.fields.step_count == eager.fields.step_count
+    for a, b in losses:
+        assert abs(a - b) <= 1e-3 * abs(a), losses
