@@ -126,3 +126,75 @@ def test_replayed_steps_move_the_matrices_as_eager_ones(dev):
     assert t.matrices.step_count == t.fields.step_count == eager.fields.step_count
     for a, b in losses:
         assert abs(a - b) <= 1e-3 * abs(a), losses
+
+
+@pytest.mark.parametrize("graphed", [False, True])
+def test_data_parallel_steps_exchange_every_group(dev, monkeypatch, graphed):
+    """Data-parallel steps with Muon, the other rank's part of a sum taken to be half of this one's: every value of every
+    group's gradients is summed once a step, its mean is what the matrices are moved by."""
+    from multimodalstudio_amd import ddp as mddp
+    from multimodalstudio_amd import graphs
+    from multimodalstudio_amd import pipeline as pl
+    cfg = pl.TrainConfig(method="grid", modalities=("rgb",), num_rays_per_modality=256, log2T=12, n_views=10, width=64,
+                         height=48, optimizer="muon")
+    t = pl.Trainer(cfg, dev)
+    t.set_step(95000)
+    summed, done = [], []
+
+    class Work:
+        def wait(self):
+            done.append(1)
+
+    def all_reduce(buf, op=None, async_op=False):
+        assert async_op and buf.is_contiguous()
+        summed.append((buf.data_ptr(), buf.numel()))
+        buf.mul_(1.5)
+        return Work()
+    monkeypatch.setattr(mddp.dist, "all_reduce", all_reduce)
+    ddp = mddp.DDP(2, bucket_bytes=1 << 16)
+    means = []
+    finish = ddp.finish_step
+
+    def spy(groups):
+        before = {id(g): g.grad.clone() for g in groups}
+        n = len(summed)
+        finish(groups)
+        late = {id(g): [(p, k) for p, k in summed[n:]] for g in groups}
+        for g in groups:
+            want = 0.5 * before[id(g)]     # summed while the backward ran: the mean is left
+            for p, k in late[id(g)]:
+                off = (p - g.grad.data_ptr()) // 4
+                if 0 <= off < g.grad.numel():
+                    want[off:off + k] = 0.75 * before[id(g)][off:off + k]
+            assert (g.grad - want).abs().max() <= 2.0 ** -22 * want.abs().max()
+        means.append([g.grad.clone() for g in groups])
+    monkeypatch.setattr(ddp, "finish_step", spy)
+    runner = graphs.GraphTrainer(t, granule=64, neighbours=0, ddp=ddp) if graphed else None
+    for k in range(5):
+        summed.clear()
+        done.clear()
+        before = [p.detach().clone() for p in t.matrices.params]
+        momenta = [m.clone() for m in t.matrices.momenta]
+        lr = 1e-3 * pl.lr_factor(t.step, cfg.max_iters)
+        if graphed:
+            runner.step()
+        else:
+            t.train_step(ddp=ddp)
+        torch.cuda.synchronize()
+        assert len(means[-1]) == 3 and len(done) == len(summed)
+        covered = sorted(summed)
+        for g in t.groups:
+            at = g.grad.data_ptr()
+            for p, n in covered:
+                if at <= p < g.grad.data_ptr() + 4 * g.grad.numel():
+                    assert p == at
+                    at = p + 4 * n
+            assert at == g.grad.data_ptr() + 4 * g.grad.numel()
+        assert all(torch.equal(g.grad, m) for g, m in zip(t.groups, means[-1]))
+        clip = min(1.0, 2.0 / (sum(float(g.grad.double().square().sum()) for g in (t.fields, t.matrices)) ** 0.5 + 1e-6))
+        for p, q, m, n in zip(before, t.matrices.params, momenta, t.matrices.momenta):
+            want = reference_step(p, q.grad, m, lr, 0.95, True, 0.01, "match_rms_adamw", clip)
+            assert float((n.double() - want[1]).norm()) <= 1e-4 * float(want[1].norm())
+            check_step(q.detach(), want[1].float(), want, torch.float32)
+    if graphed:
+        assert runner.disabled is None and runner.stats["replays"] >= 2, (runner.disabled, runner.stats)
