@@ -10,11 +10,13 @@
 // symmetric: only tiles on or below the diagonal are computed, the others are written as mirrors -- 3 r^2 c + r^3
 // floating-point operations a step in place of 4 r^2 c + 2 r^3.
 //
-// What bounds it.  Large matrices: the products, at the rate the card's power allows (4096 x 4096, prec 1: 1.39 .. 1.46
-// ms, 940 .. 990 TFLOP/s of the operations above; a library product of that size reaches 1040); prec 0 does three products
-// for one (a 2048-wide block of six matrices: 4.27 .. 4.54 ms, 980 .. 1040 TFLOP/s of its fp16 products).  Stacks of 1024 x
-// 4096: the iterates' way through memory beside them (8 bytes an element and step, with the operand 10).  Small ones: 2 +
-// 3 steps launches of 4 to 8 us, each one block's loads, products and stores in a row (the renderer's 19 matrices: 130 us).
+// What bounds it.  Large matrices: the products, at the rate the card's power allows (4096 x 4096: prec 0, three products
+// for one, 3.27 .. 3.45 ms, 1190 .. 1260 TFLOP/s of its fp16 products; prec 1 1.34 .. 1.46 ms, 940 .. 1025; a library
+// product reaches 1040 .. 1110 at that size, 1308 at 8192; a 2048-wide block of six matrices, prec 0: 4.34 .. 4.56 ms,
+// 975 .. 1025).
+// Stacks of 1024 x 4096: the iterates' way through memory beside them (prec 1: 8 bytes an element and step, with the
+// operand 10).  Small ones: 2 + 3 steps launches of 4 to 8 us, each one block's loads, products and stores in a row (the
+// renderer's 19 matrices: 131 us).
 //
 // Precision.  Operands are fp16, X, A and B each times the largest power of two that its entries allow: they are bounded
 // by singular values, those by the coefficients (2^15 X, 2^15 A, 2^14 B for a, b, c = 3.4445, -4.7750, 2.0315); fp32
@@ -26,8 +28,9 @@
 //           and a unit of 2^10 for all: 1.8e-5; float32 products 0.8e-7).  bf16 pairs hold 16 bits only, which the
 //           map's slope (up to a^5 = 485 for small singular values) takes to 3e-5 .. 2e-4.
 //   prec 1  one fp16 product.  X itself keeps hi + lo and a X is added from those in fp32: rounding only enters
-//           through (b A + c A A) X, so the result is 0.9e-3 .. 1.4e-3 off, under bf16's own 1.7e-3 (X rounded to fp16
-//           between steps: up to 1.2e-2 where a few directions are far stronger than the rest).  Matrices of up to 128
+//           through (b A + c A A) X, so the result is 0.6e-3 .. 1.6e-3 off, under bf16's own 1.7e-3 (3e-3 where one
+//           entry stands for nearly all of the norm; X rounded to fp16 between steps: up to 1.2e-2 where a few
+//           directions are far stronger than the rest).  Matrices of up to 128
 //           rows or columns run prec 0 all the same: they wait for launches and loads, not for products, and with few
 //           entries to average over, single products are up to 3.8e-3 off.
 //
@@ -1044,7 +1047,7 @@ bool overlap(const Rows& a, const Rows& b) {
   const Rows &few = a.rows * a.batch <= b.rows * b.batch ? a : b, &many = &few == &a ? b : a;
   // columns of one buffer, side by side
   if (a.ld == b.ld && a.bs % a.ld == 0 && b.bs % a.ld == 0) {
-    const int64_t d = many.lo >= few.lo ? (int64_t)(many.lo - few.lo) % a.ld : (a.ld - (int64_t)(few.lo - many.lo) % a.ld) % a.ld;
+    const int64_t from = (int64_t)(many.lo - few.lo) % a.ld, d = from < 0 ? from + a.ld : from;
     if (d >= few.width && d + many.width <= a.ld) return false;
   }
   for (int64_t k = 0; k < few.batch; ++k)
