@@ -131,6 +131,7 @@ class FlatGroup:
         self.v = torch.zeros(n + pad, device=dev)
         self.sumsq = torch.zeros(1, device=dev)
         self.norm_groups: Optional[List[FlatGroup]] = None   # whose gradients' norm the clip goes by, if not its own's
+        self.banked = False         # an OptimBank holds the address of sumsq
         # this step's AdamW scalars for graph replays (mms_adamw_dev; layout of mms_adamw_scalars)
         self.hyper = torch.zeros(8, device=dev)
         # two pinned staging buffers, alternated: a step's scalars can be queued behind the previous replay while
@@ -209,6 +210,8 @@ class FlatGroup:
 def clip_together(groups: Sequence["FlatGroup"]) -> None:
     """One clip for several groups: each goes by the norm of all their gradients, as clip_grad_norm_ over their
     parameters (before an OptimBank is made of them)."""
+    if any(g.banked for g in groups):
+        raise ValueError("clip_together: a group is in an OptimBank already")
     for g in groups:
         g.sumsq, g.norm_groups = groups[0].sumsq, list(groups)
 
@@ -279,6 +282,7 @@ class OptimBank:
         self.hyper = torch.zeros(G * 8, device=dev)
         for i, g in enumerate(self.groups):
             g.hyper = self.hyper[8 * i:8 * i + 8]
+            g.banked = True
         self._hyper_host = [torch.zeros(G * 8).pin_memory() if dev.type == "cuda" else torch.zeros(G * 8)
                             for _ in range(2)]
         self._hyper_slot = 0

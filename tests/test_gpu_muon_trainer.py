@@ -72,6 +72,9 @@ def test_no_clip_and_a_torn_bank(dev):
         check_step(p.detach(), m, w, torch.float32)
     with pytest.raises(ValueError, match="bank"):
         pl.OptimBank([mu])
+    pl.OptimBank([ad, mu])
+    with pytest.raises(ValueError, match="OptimBank"):
+        pl.clip_together([ad, mu])
 
 
 def test_the_trainer_clips_as_with_adamw(dev):
